@@ -56,7 +56,10 @@ HIP_FLAGS = [
 ]
 
 # per-translation-unit extra flags of the kernel library (A/B builds: AMDK8S_HIP_DEFINES)
-FILE_FLAGS: dict = {}
+FILE_FLAGS: dict = {
+    # no packed fp32 instructions: some of their forms have given wrong results on these cards
+    "llm_kv8.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
+}
 
 
 @dataclass

@@ -1,0 +1,1397 @@
+// Paged KV cache in 8 bits and the attention that reads it (LLM serving), gfx950.
+//
+// A page holds 64 positions of every KV head; each (page, head) has one key scale and one value scale:
+//   k  [pages][Hkv][64][D]   key codes, position-major         K[j] = ks code
+//   v  [pages][Hkv][D][64]   value codes, dim-major            V[j] = vs code
+//   ks, vs [pages][Hkv]      fp32, powers of two: the least 2^e with amax <= qmax 2^e (int8 127,
+//                            e4m3 448); 0 for an all-zero block, NaN for one with a non-finite value
+// Values lie dim-major because the P.V matrix instruction takes, for one dim, consecutive positions of
+// a lane: both products then read the cache in the order their operands need it, straight from memory
+// (decode) or with plain LDS reads (prompt), and nothing is transposed on the way.
+// Scales are powers of two so that code x scale is exact in bf16 and a scale that has to grow (a larger
+// value arrives in a begun page) shifts the old codes: an e4m3 page loses only subnormals by it, an
+// int8 page at most 1/2 + 1/4 + ... < 1 step however often it grows (with scales of amax / 127 every
+// growth would round anew).  The price is a step up to twice as large as amax / 127.
+//
+// A sequence is a row of the page table; an entry outside the pool (-1) is an unmapped page: what
+// would be written there is dropped, and its positions are not attended.  Query p sees key j when
+//   j <= p  and  (window == 0 or j > p - window or j < sinks).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+namespace {
+
+constexpr int kPage = 64;
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+enum { kF16 = 0, kBF16 = 1, kF32 = 2 };
+
+// ---------------------------------------------------------------- 16-bit and 8-bit types
+template <int T>
+struct Elem;
+template <>
+struct Elem<kF16> {
+  typedef uint16_t type;
+  static __device__ __forceinline__ float get(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
+  static __device__ __forceinline__ uint16_t put(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+};
+template <>
+struct Elem<kBF16> {
+  typedef uint16_t type;
+  static __device__ __forceinline__ float get(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+  static __device__ __forceinline__ uint16_t put(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+};
+template <>
+struct Elem<kF32> {
+  typedef float type;
+  static __device__ __forceinline__ float get(float x) { return x; }
+  static __device__ __forceinline__ float put(float x) { return x; }
+};
+
+// N consecutive elements as floats; `wide`: the address is a multiple of 16 bytes (uniform)
+template <int T, int N>
+__device__ __forceinline__ void load_n(const typename Elem<T>::type* p, bool wide, float (&x)[N]) {
+  typedef typename Elem<T>::type E;
+  constexpr int PER = 16 / sizeof(E);
+  if (wide) {
+#pragma unroll
+    for (int c = 0; c < N / PER; ++c) {
+      const uint4 w = reinterpret_cast<const uint4*>(p)[c];
+      E e[PER];
+      __builtin_memcpy(e, &w, 16);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[c * PER + i] = Elem<T>::get(e[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = Elem<T>::get(p[i]);
+  }
+}
+template <int T, int N>
+__device__ __forceinline__ void store_n(typename Elem<T>::type* p, bool wide, const float (&x)[N]) {
+  typedef typename Elem<T>::type E;
+  constexpr int PER = 16 / sizeof(E);
+  if (wide) {
+#pragma unroll
+    for (int c = 0; c < N / PER; ++c) {
+      E e[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) e[i] = Elem<T>::put(x[c * PER + i]);
+      uint4 w;
+      __builtin_memcpy(&w, e, 16);
+      reinterpret_cast<uint4*>(p)[c] = w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = Elem<T>::put(x[i]);
+  }
+}
+
+// four codes of one dword as fp16 pairs (exact: |int8| < 2^11, e4m3 has 4 significant bits and fp16's
+// exponent range).  int8: the byte with its sign flipped is code + 128; under the high byte 0x64 it
+// reads as the fp16 1024 + 128 + code, and one packed subtraction leaves the code.
+template <bool FP8>
+__device__ __forceinline__ void codes_h4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FP8) {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+  } else {
+    const uint32_t u = w ^ 0x80808080u;
+    const h2 bias = {(_Float16)1152.f, (_Float16)1152.f};
+    const uint32_t a = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+    const uint32_t b = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, a) - bias);
+    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, b) - bias);
+  }
+}
+// eight codes (two dwords) as the eight fp16 of a matrix operand
+template <bool FP8>
+__device__ __forceinline__ h8 codes_h8(uint32_t a, uint32_t b) {
+  uint4 r;
+  codes_h4<FP8>(a, r.x, r.y);
+  codes_h4<FP8>(b, r.z, r.w);
+  return __builtin_bit_cast(h8, r);
+}
+template <bool FP8>
+__device__ __forceinline__ void codes_f4(uint32_t w, float (&x)[4]) {
+  if constexpr (FP8) {
+    const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));
+  }
+}
+// four values (already divided by the scale) to codes, ties to even
+template <bool FP8>
+__device__ __forceinline__ uint32_t to_codes4(float a, float b, float c, float d) {
+  if constexpr (FP8) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+  } else {
+    return ((uint32_t)(int)__builtin_rintf(a) & 0xffu) | (((uint32_t)(int)__builtin_rintf(b) & 0xffu) << 8) |
+           (((uint32_t)(int)__builtin_rintf(c) & 0xffu) << 16) | ((uint32_t)(int)__builtin_rintf(d) << 24);
+  }
+}
+template <bool FP8>
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
+  float x[4];
+  codes_f4<FP8>(w, x);
+  return to_codes4<FP8>(x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio);
+}
+
+// the least 2^e with amax <= qmax 2^e, from amax's bits (>= 0; NaN and infinity have the largest)
+template <bool FP8>
+__device__ __forceinline__ float block_scale(uint32_t bits) {
+  if (bits == 0) return 0.f;
+  if (bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  const int ex = (int)(bits >> 23) - 127;              // a subnormal amax falls under the floor below
+  // qmax = 1.984375 x 2^6 (127) or 1.75 x 2^8 (448): one more when the significand passes it
+  const int e = FP8 ? ex - 8 + ((bits & 0x7fffffu) > 0x600000u) : ex - 6 + ((bits & 0x7fffffu) > 0x7e0000u);
+  return __uint_as_float((uint32_t)(max(e, -100) + 127) << 23);
+}
+
+// ---------------------------------------------------------------- ragged segments
+// Sequence s has rows cu[s] .. cu[s + 1] - 1 at positions start[s] ..; what is out of order, out of
+// [0, N) or at a negative start counts as empty.
+struct Segs {
+  const int* start;
+  const int* cu;
+  int S, N;
+  __device__ __forceinline__ void get(int s, int& row, int& n, int& pos) const {
+    row = max(cu[s], 0);
+    n = min(cu[s + 1], N) - row;
+    pos = start[s];
+    if (pos < 0 || pos > 0x3fffffff) n = 0;
+  }
+};
+
+// The unit'th piece of all segments, each cut into pieces by `count` (pieces of segment s); the whole
+// wave calls it and gets the same answer.  False: there are fewer pieces.
+template <typename F>
+__device__ __forceinline__ bool find_piece(const Segs& sg, int unit, F count, int& s, int& piece) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int base = 0; base < sg.S; base += 64) {
+    int c = 0;
+    if (base + lane < sg.S) {
+      int row, n, pos;
+      sg.get(base + lane, row, n, pos);
+      c = n > 0 ? count(n, pos) : 0;
+    }
+    int inc = c;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += up;
+    }
+    const uint64_t past = __ballot(before + inc > unit);
+    if (past) {
+      const int hit = __builtin_ctzll(past);
+      s = __builtin_amdgcn_readfirstlane(base + hit);
+      piece = __builtin_amdgcn_readfirstlane(unit - before - (__shfl(inc, hit, 64) - __shfl(c, hit, 64)));
+      return true;
+    }
+    before += __shfl(inc, 63, 64);
+  }
+  return false;
+}
+
+// The segment of row n (the whole wave asks for one row) and the row's position; false: in none.
+__device__ __forceinline__ bool find_row(const Segs& sg, int n, int& pos) {
+  const int lane = threadIdx.x & 63;
+  int s = 0;                                             // segments that end at or before row n
+  for (int base = 0; base < sg.S; base += 64)
+    s += __builtin_popcountll(__ballot(base + lane < sg.S && sg.cu[base + lane + 1] <= n));
+  s = __builtin_amdgcn_readfirstlane(s);
+  if (s >= sg.S) return false;
+  int row, cnt;
+  sg.get(s, row, cnt, pos);
+  pos += n - row;
+  return n >= row && n < row + cnt;
+}
+
+__device__ __forceinline__ int pages_of(int n, int pos) { return (pos + n - 1) / kPage - pos / kPage + 1; }
+
+// most pieces of `each` rows (pages: of any alignment) that N rows in S segments make
+inline long most_pages(long N, long S) {
+  const long m = (N + 62 * S) / 64 + S;
+  return m < N ? m : N;
+}
+
+struct Pool {
+  uint8_t* k;
+  uint8_t* v;
+  float* ks;
+  float* vs;
+  const int* table;
+  int pool, Hkv, width, stride;        // pages in the pool; table columns and row stride
+  __device__ __forceinline__ int page(int s, int j) const {
+    if ((unsigned)j >= (unsigned)width) return -1;
+    const int id = table[(long)s * stride + j];
+    return (unsigned)id < (unsigned)pool ? id : -1;
+  }
+};
+
+// ---------------------------------------------------------------- append
+struct AppendArgs {
+  Pool c;
+  Segs sg;
+  const void* k;
+  const void* v;
+  const void* q;
+  void* qo;
+  const float* cos_t;
+  const float* sin_t;
+  long sk_tok, sk_head, sv_tok, sv_head, sq_tok, sq_head, so_tok, so_head;
+  int H, units, table_rows;            // table_rows: rows of the rotation tables
+  bool wide_kv, wide_q;
+};
+
+// a rounding after every operation (the compiler would fuse the products into one fma otherwise)
+__device__ __forceinline__ float turn_lo(float a, float b, float c, float s) {
+#pragma clang fp contract(off)
+  const float x = a * c, y = b * s;
+  return x - y;
+}
+__device__ __forceinline__ float turn_hi(float a, float b, float c, float s) {
+#pragma clang fp contract(off)
+  const float x = a * s, y = b * c;
+  return x + y;
+}
+
+// eight pairs (d, d + D/2) of one row: rotated in fp32 with a rounding after every operation (one
+// definition of the rotated key's bits, whoever computes it)
+template <int T, int D>
+__device__ __forceinline__ void load_turned(const typename Elem<T>::type* row, bool wide, const float* cos_t,
+                                            const float* sin_t, long pos, int d0, float (&lo)[8], float (&hi)[8]) {
+  float a[8], b[8];
+  load_n<T, 8>(row + d0, wide, a);
+  load_n<T, 8>(row + D / 2 + d0, wide, b);
+  if (cos_t) {
+    float c[8], s[8];
+    load_n<kF32, 8>(cos_t + pos * (D / 2) + d0, true, c);
+    load_n<kF32, 8>(sin_t + pos * (D / 2) + d0, true, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      lo[i] = turn_lo(a[i], b[i], c[i], s[i]);
+      hi[i] = turn_hi(a[i], b[i], c[i], s[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { lo[i] = a[i]; hi[i] = b[i]; }
+  }
+}
+
+// Blocks [0, units * Hkv): one page of one sequence and KV head each, 256 threads: the new rows' keys
+// are rotated, the page's new scale is the larger of the old one (if the page was begun before) and
+// the new rows' own, old codes are shifted if it grew, the new rows' codes are written.  One block owns
+// the page's codes and scales, so there are no atomics.  The blocks behind rotate the queries, a wave a
+// row.  Memory-bound: 16-byte loads and stores of whole rows; a value code row of 64 positions is
+// written in 16-byte pieces through an LDS transpose.
+template <int D, bool FP8, int T, int TO>
+__global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
+  typedef typename Elem<T>::type E;
+  constexpr int PR = D / 16;                             // 8-pair items of a row
+  constexpr int PER = kPage * PR / 256;                  // items a thread
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if ((int)blockIdx.x >= a.units * a.c.Hkv) {            // ---- queries
+    const int n = ((int)blockIdx.x - a.units * a.c.Hkv) * 4 + wave;
+    if (n >= a.sg.N) return;
+    int pos;
+    if (!find_row(a.sg, n, pos)) return;
+    if (pos >= a.table_rows) return;
+    const E* q = static_cast<const E*>(a.q) + (long)n * a.sq_tok;
+    typedef typename Elem<TO>::type EO;
+    EO* o = static_cast<EO*>(a.qo) + (long)n * a.so_tok;
+    for (int i = lane; i < a.H * PR; i += 64) {
+      const int h = i / PR, d0 = 8 * (i % PR);
+      float lo[8], hi[8];
+      load_turned<T, D>(q + h * a.sq_head, a.wide_q, a.cos_t, a.sin_t, pos, d0, lo, hi);
+      store_n<TO, 8>(o + h * a.so_head + d0, a.wide_q, lo);
+      store_n<TO, 8>(o + h * a.so_head + D / 2 + d0, a.wide_q, hi);
+    }
+    return;
+  }
+  __shared__ uint32_t red[2][4];
+  __shared__ __align__(16) uint8_t img[kPage][D + 16];   // value codes by position
+  const int kh = blockIdx.x % a.c.Hkv;
+  int s, piece;
+  if (!find_piece(a.sg, blockIdx.x / a.c.Hkv, [](int n, int p) { return pages_of(n, p); }, s, piece)) return;
+  int row, cnt, pos;
+  a.sg.get(s, row, cnt, pos);
+  const int j = pos / kPage + piece;
+  const int id = a.c.page(s, j);
+  if (id < 0) return;
+  const int r0 = max(pos - j * kPage, 0), r1 = min(pos + cnt - j * kPage, kPage);   // new rows
+  const long n0 = (long)row + j * kPage - pos;           // input row of the page's position 0
+  const long sc = (long)id * a.c.Hkv + kh;
+  uint8_t* kc = a.c.k + sc * kPage * D;
+  uint8_t* vc = a.c.v + sc * kPage * D;
+  const float oldk = r0 ? a.c.ks[sc] : 0.f, oldv = r0 ? a.c.vs[sc] : 0.f;
+  const E* kin = static_cast<const E*>(a.k) + kh * a.sk_head;
+  const E* vin = static_cast<const E*>(a.v) + kh * a.sv_head;
+  float klo[PER][8], khi[PER][8], vlo[PER][8], vhi[PER][8];
+  uint32_t mk = 0, mv = 0;                               // largest magnitudes, as bits (NaN largest)
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int i = tid + 256 * u, r = i / PR, d0 = 8 * (i % PR);
+    if (r >= r0 && r < r1) {
+      const long n = n0 + r;
+      load_turned<T, D>(kin + n * a.sk_tok, a.wide_kv, a.cos_t, a.sin_t, (long)j * kPage + r, d0, klo[u], khi[u]);
+      load_n<T, 8>(vin + n * a.sv_tok + 2 * d0, a.wide_kv, vlo[u]);
+      load_n<T, 8>(vin + n * a.sv_tok + 2 * d0 + 8, a.wide_kv, vhi[u]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        mk = max(mk, max(__float_as_uint(klo[u][e]) & 0x7fffffffu, __float_as_uint(khi[u][e]) & 0x7fffffffu));
+        mv = max(mv, max(__float_as_uint(vlo[u][e]) & 0x7fffffffu, __float_as_uint(vhi[u][e]) & 0x7fffffffu));
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    mk = max(mk, (uint32_t)__shfl_xor((int)mk, o, 64));
+    mv = max(mv, (uint32_t)__shfl_xor((int)mv, o, 64));
+  }
+  if (lane == 0) { red[0][wave] = mk; red[1][wave] = mv; }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) { mk = max(mk, red[0][w]); mv = max(mv, red[1][w]); }
+  // the larger of both, NaN above all (scales are never negative: their bits order like they do)
+  const float nk = __uint_as_float(max(__float_as_uint(block_scale<FP8>(mk)), __float_as_uint(oldk)));
+  const float nv = __uint_as_float(max(__float_as_uint(block_scale<FP8>(mv)), __float_as_uint(oldv)));
+  const float ik = nk > 0.f ? 1.f / nk : 0.f, iv = nv > 0.f ? 1.f / nv : 0.f;
+  const bool badk = nk != nk, badv = nv != nv;
+  const bool growk = r0 && nk > oldk, growv = r0 && nv > oldv;   // (a NaN block keeps its codes)
+  if (tid == 0) { a.c.ks[sc] = nk; a.c.vs[sc] = nv; }
+  if (growk) {
+    const float ratio = oldk * ik;
+    for (int i = tid; i < r0 * (D / 16); i += 256) {
+      uint4 w = reinterpret_cast<uint4*>(kc)[i];
+      w.x = rescale4<FP8>(w.x, ratio); w.y = rescale4<FP8>(w.y, ratio);
+      w.z = rescale4<FP8>(w.z, ratio); w.w = rescale4<FP8>(w.w, ratio);
+      reinterpret_cast<uint4*>(kc)[i] = w;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int i = tid + 256 * u, r = i / PR, d0 = 8 * (i % PR);
+    if (r >= r0 && r < r1) {
+      uint2 w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        klo[u][e] = badk ? 0.f : klo[u][e] * ik;
+        khi[u][e] = badk ? 0.f : khi[u][e] * ik;
+        vlo[u][e] = badv ? 0.f : vlo[u][e] * iv;
+        vhi[u][e] = badv ? 0.f : vhi[u][e] * iv;
+      }
+      w.x = to_codes4<FP8>(klo[u][0], klo[u][1], klo[u][2], klo[u][3]);
+      w.y = to_codes4<FP8>(klo[u][4], klo[u][5], klo[u][6], klo[u][7]);
+      *reinterpret_cast<uint2*>(kc + r * D + d0) = w;
+      w.x = to_codes4<FP8>(khi[u][0], khi[u][1], khi[u][2], khi[u][3]);
+      w.y = to_codes4<FP8>(khi[u][4], khi[u][5], khi[u][6], khi[u][7]);
+      *reinterpret_cast<uint2*>(kc + r * D + D / 2 + d0) = w;
+      uint4 x;
+      x.x = to_codes4<FP8>(vlo[u][0], vlo[u][1], vlo[u][2], vlo[u][3]);
+      x.y = to_codes4<FP8>(vlo[u][4], vlo[u][5], vlo[u][6], vlo[u][7]);
+      x.z = to_codes4<FP8>(vhi[u][0], vhi[u][1], vhi[u][2], vhi[u][3]);
+      x.w = to_codes4<FP8>(vhi[u][4], vhi[u][5], vhi[u][6], vhi[u][7]);
+      *reinterpret_cast<uint4*>(&img[r][2 * d0]) = x;
+    }
+  }
+  __syncthreads();
+  const float rv = growv ? oldv * iv : 1.f;
+  for (int i = tid; i < D * 4; i += 256) {               // 16 positions of one dim
+    const int d = i % D, p0 = 16 * (i / D);
+    const bool has_new = p0 < r1 && p0 + 16 > r0;
+    if (!has_new && !(growv && p0 < r0)) continue;
+    uint4* at = reinterpret_cast<uint4*>(vc + d * kPage + p0);
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (p0 < r0 || p0 + 16 > r1) {                       // some of them are not new
+      const uint4 old = *at;
+      w[0] = old.x; w[1] = old.y; w[2] = old.z; w[3] = old.w;
+      if (growv) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = rescale4<FP8>(w[e], rv);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int r = p0 + e;
+      if (r >= r0 && r < r1)
+        w[e >> 2] = (w[e >> 2] & ~(0xffu << (8 * (e & 3)))) | ((uint32_t)img[r][d] << (8 * (e & 3)));
+    }
+    *at = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// ---------------------------------------------------------------- read
+struct ReadArgs {
+  Pool c;
+  Segs sg;
+  void* ko;
+  void* vo;
+  long sk_tok, sk_head, sv_tok, sv_head;
+  bool wide;
+};
+
+// one page of one sequence and KV head a block: keys row by row, values through an LDS transpose
+template <int D, bool FP8, int T>
+__global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
+  typedef typename Elem<T>::type E;
+  __shared__ __align__(16) uint8_t img[kPage][D + 16];
+  const int tid = threadIdx.x;
+  const int kh = blockIdx.x % a.c.Hkv;
+  int s, piece;
+  if (!find_piece(a.sg, blockIdx.x / a.c.Hkv, [](int n, int p) { return pages_of(n, p); }, s, piece)) return;
+  int row, cnt, pos;
+  a.sg.get(s, row, cnt, pos);
+  const int j = pos / kPage + piece;
+  const int r0 = max(pos - j * kPage, 0), r1 = min(pos + cnt - j * kPage, kPage);
+  const long n0 = (long)row + j * kPage - pos;
+  const int id = a.c.page(s, j);
+  const bool live = id >= 0;
+  const long sc = (long)max(id, 0) * a.c.Hkv + kh;
+  const uint8_t* kc = a.c.k + sc * kPage * D;
+  const uint8_t* vc = a.c.v + sc * kPage * D;
+  const float sk = live ? a.c.ks[sc] : 0.f, sv = live ? a.c.vs[sc] : 0.f;
+  for (int i = tid; i < D * 4; i += 256) {               // 16 positions of one dim
+    const int d = i % D, p0 = 16 * (i / D);
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (live && p0 < r1 && p0 + 16 > r0) x = *reinterpret_cast<const uint4*>(vc + d * kPage + p0);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) img[p0 + e][d] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+  }
+  __syncthreads();
+  for (int i = tid; i < kPage * (D / 16); i += 256) {
+    const int r = i / (D / 16), d0 = 16 * (i % (D / 16));
+    if (r < r0 || r >= r1) continue;
+    const uint4 kx = live ? *reinterpret_cast<const uint4*>(kc + r * D + d0) : make_uint4(0, 0, 0, 0);
+    const uint4 vx = *reinterpret_cast<const uint4*>(&img[r][d0]);
+    float y[16], x[4];
+    const uint32_t kw[4] = {kx.x, kx.y, kx.z, kx.w}, vw[4] = {vx.x, vx.y, vx.z, vx.w};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      codes_f4<FP8>(kw[c], x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[4 * c + e] = x[e] * sk;
+    }
+    store_n<T, 16>(static_cast<E*>(a.ko) + (n0 + r) * a.sk_tok + kh * a.sk_head + d0, a.wide, y);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      codes_f4<FP8>(vw[c], x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[4 * c + e] = x[e] * sv;
+    }
+    store_n<T, 16>(static_cast<E*>(a.vo) + (n0 + r) * a.sv_tok + kh * a.sv_head + d0, a.wide, y);
+  }
+}
+
+// ---------------------------------------------------------------- attention, both forms
+// The pages that queries at positions lo .. hi see, as a list: the first `sinks` ones, then those from
+// `first` on.
+struct Seen {
+  int nsink, first, n;
+  __device__ __forceinline__ int page(int i) const { return i < nsink ? i : first + i - nsink; }
+};
+__host__ __device__ __forceinline__ Seen seen_pages(int lo, int hi, int span, int window, int sinks) {
+  Seen s{0, 0, 0};
+  const int end = hi < span ? hi + 1 : span;             // keys below `end`
+  if (end <= 0) return s;
+  const int last = (end + kPage - 1) / kPage;
+  if (window > 0) {
+    const int low = lo - window + 1;
+    s.first = low > 0 ? low / kPage : 0;
+    if (s.first > last) s.first = last;
+    const int ns = sinks < end ? (sinks + kPage - 1) / kPage : last;
+    s.nsink = ns < s.first ? ns : s.first;
+  }
+  s.n = s.nsink + last - s.first;
+  return s;
+}
+
+// x of lane l ^ 16 / l ^ 32 on the VALU
+__device__ __forceinline__ float xor16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float((threadIdx.x & 16) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float xor32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// log2 of a page's value scale over the reference `vref` (the largest so far, > 0 unless all were 0).
+// The weights p = 2^(s - m) go to the matrix instruction as fp16 p vs / vref, so that pages of unlike
+// scales add up in one accumulator; the sum of the plain p's takes the factor back (`back`).  A zero
+// page has zero codes: any weight will do.  A NaN scale stays.  What the rounding costs: 2^-12 of a
+// weight, and weights below 2^-24 (of the largest weight times the largest value scale) are lost.
+__device__ __forceinline__ float value_weight(float vs, float vref, float& back) {
+  if (vs == 0.f) { back = 1.f; return 0.f; }
+  float lw = __builtin_amdgcn_logf(vs / vref);
+  lw = lw < -60.f ? -60.f : lw;                          // no fp16 weight is left there anyway
+  back = __builtin_amdgcn_exp2f(-lw);
+  return lw;
+}
+
+// a power of two f so that x f (|x| <= amax) has fp16's range to spare: amax f in [2^8, 2^9)
+__device__ __forceinline__ float fit_f16(float amax) {
+  const int ex = (int)((__float_as_uint(amax) >> 23) & 0xff);
+  return ex == 0 || ex == 255 ? 1.f : __uint_as_float((uint32_t)(min(max(262 - ex, 1), 254)) << 23);
+}
+
+struct AttnArgs {
+  Pool c;
+  Segs sg;                 // prompt; decode: start = positions, N = S
+  const uint16_t* q;
+  void* out;               // null: only q8
+  float* po;               // partial outputs [parts][rows][H][D], rows = N
+  float* pml;              // [parts][rows][H][2] (max in log2 units, sum)
+  int8_t* x8;              // Q8 output (decode): [N][H D], scales of 32, scaled sums of 16
+  float* dx;
+  float* sx;
+  long sq_tok, sq_head, so_tok, so_head;
+  int H, G, span, window, sinks, parts, units;
+  float c2;                // scale x log2(e)
+  bool wide_q, wide_o;
+};
+
+// pages a workgroup streams, and workgroups (partials) of a token that sees n pages: its own count
+// decides, so that its bits do not depend on the batch
+constexpr int kDecWaves = 4;
+constexpr int kDecParts = 64;
+constexpr int kDecMaxPer = 64;                           // pages a wave (a lane holds one page's table entry)
+__host__ __device__ __forceinline__ int dec_per_wave(int n) {
+  int p = 1;
+  while (p < kDecMaxPer && n > kDecParts * kDecWaves * p) p <<= 1;
+  return p;
+}
+__host__ __device__ __forceinline__ int dec_parts(int n) {
+  const int w = kDecWaves * dec_per_wave(n);
+  return (n + w - 1) / w;
+}
+inline int dec_parts_most(int n) {                       // of any count <= n
+  int m = dec_parts(n);
+  for (int e = kDecParts * kDecWaves; e < n; e <<= 1) {
+    const int p = dec_parts(e);
+    if (p > m) m = p;
+  }
+  return m;
+}
+
+// Single-token attention.  Grid (Hkv x groups of 16 heads, parts, S); a wave streams whole pages with
+// its own online softmax, no LDS and no barrier until the waves merge.  Both products on
+// v_mfma_f32_16x16x32_f16, operands straight from memory:
+// * S = K q^T: tile t of four has the rows m = 0..15 at positions 16 (m >> 2) + 4 t + (m & 3), so that
+//   lane (head pr, group kg) gets the scores of positions 16 kg .. 16 kg + 15 over the four tiles;
+// * O^T = V^T P^T: the value codes lie dim-major, a lane's 16 bytes are positions 16 kg .. + 15 of one
+//   dim: the same positions as its scores, so neither P nor V moves between lanes.  The running
+//   maximum, sum and rescaling are one head's, a lane's own.
+template <int D, bool FP8, int T>
+__global__ void __launch_bounds__(64 * kDecWaves) kv8_decode_kernel(const AttnArgs a) {
+  constexpr int NW = kDecWaves, KH = D / 64, ND = D / 16;
+  const int hg = (a.G + 15) / 16;
+  const int kh = blockIdx.x / hg, h0 = (blockIdx.x % hg) * 16;
+  const int part = blockIdx.y, t = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pr = lane & 15, kg = lane >> 4;
+  const int gn = min(16, a.G - h0);                      // heads of this workgroup
+  const int pos = a.sg.start[t];
+  const Seen seen = seen_pages(pos, pos, a.span, a.window, a.sinks);
+  const int per = dec_per_wave(seen.n);
+  const int p0 = part * per * NW;
+  if (p0 >= seen.n && part > 0) return;                  // part 0 of an empty row writes its zeros
+  const int mine = max(0, min(per, (seen.n - p0 - wave + NW - 1) / NW));   // pages p0 + wave + NW i
+
+  // lane i: table entry and scales of this wave's i'th page
+  int my_id = -1;
+  float my_ks = 0.f, my_vs = 0.f;
+  if (lane < mine) {
+    my_id = a.c.page(t, seen.page(p0 + wave + NW * lane));
+    if (my_id >= 0) {
+      const long sc = (long)my_id * a.c.Hkv + kh;
+      my_ks = a.c.ks[sc];
+      my_vs = a.c.vs[sc];
+    }
+  }
+  uint4 kb[2][4 * KH], vb[2][ND];
+  auto load_page = [&](int i, uint4 (&kr)[4 * KH], uint4 (&vr)[ND]) __attribute__((always_inline)) {
+    const int id = max(__builtin_amdgcn_readlane(my_id, i), 0);
+    const long base = ((long)id * a.c.Hkv + kh) * kPage * D;
+    const uint8_t* kp = a.c.k + base + (16 * (pr >> 2) + (pr & 3)) * D + 16 * kg;
+    const uint8_t* vp = a.c.v + base + pr * kPage + 16 * kg;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int h = 0; h < KH; ++h) kr[u * KH + h] = *reinterpret_cast<const uint4*>(kp + 4 * u * D + 64 * h);
+#pragma unroll
+    for (int n = 0; n < ND; ++n) vr[n] = *reinterpret_cast<const uint4*>(vp + 16 * n * kPage);
+  };
+  if (mine > 0) load_page(0, kb[0], vb[0]);
+
+  // q operand: head pr, dims 64 h + 16 kg + 8 u + 0..7 (the order in which the key bytes lie)
+  h8 qa[2 * KH];
+  float qf = a.c2;
+  {
+    const uint16_t* qr = a.q + (long)t * a.sq_tok + (long)(kh * a.G + h0 + min(pr, gn - 1)) * a.sq_head;
+    float x[KH][16], amax = 0.f;
+#pragma unroll
+    for (int h = 0; h < KH; ++h) {
+      load_n<T, 16>(qr + 64 * h + 16 * kg, a.wide_q, x[h]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[h][e]));
+    }
+    float f = 1.f;
+    if constexpr (T == kBF16) {                          // bf16 to fp16: exact after a shift by head
+      amax = fmaxf(amax, xor16(amax));
+      amax = fmaxf(amax, xor32(amax));
+      f = fit_f16(amax);
+      qf /= f;
+    }
+#pragma unroll
+    for (int h = 0; h < KH; ++h)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qa[2 * h + u][e] = (_Float16)(x[h][8 * u + e] * f);
+  }
+
+  float m = -INFINITY, l = 0.f, vref = 0.f;
+  f4 o[ND];
+#pragma unroll
+  for (int n = 0; n < ND; ++n) o[n] = f4{0.f, 0.f, 0.f, 0.f};
+
+  auto use_page = [&](int i, uint4 (&kr)[4 * KH], uint4 (&vr)[ND]) __attribute__((always_inline)) {
+    if (__builtin_amdgcn_readlane(my_id, i) < 0) return;
+    const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_ks), i));
+    const float vs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_vs), i));
+    const int base = seen.page(p0 + wave + NW * i) * kPage;
+    f4 acc[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      acc[u] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < KH; ++h) {
+        const uint4 w = kr[u * KH + h];
+        acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h8<FP8>(w.x, w.y), qa[2 * h], acc[u], 0, 0, 0);
+        acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h8<FP8>(w.z, w.w), qa[2 * h + 1], acc[u], 0, 0, 0);
+      }
+    }
+    const float f = ks * qf;
+    float sc[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[e] = acc[e >> 2][e & 3] * f;
+    const int last = min(pos, a.span - 1);
+    const bool whole = base + kPage - 1 <= last &&
+                       (a.window <= 0 || base > pos - a.window || base + kPage <= a.sinks);
+    if (!whole) {                                        // a border inside the page (wave-uniform)
+      uint32_t keep[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int j = base + 16 * kg + e;
+        const bool in = j <= last && (a.window <= 0 || j > pos - a.window || j < a.sinks);
+        sc[e] = in ? sc[e] : -INFINITY;
+        keep[e >> 2] |= in ? 0xffu << (8 * (e & 3)) : 0u;
+      }
+#pragma unroll
+      for (int n = 0; n < ND; ++n) {                     // codes never written may be NaN: 0 x NaN
+        vr[n].x &= keep[0]; vr[n].y &= keep[1]; vr[n].z &= keep[2]; vr[n].w &= keep[3];
+      }
+    }
+    float mx = sc[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+    if (vs > vref) {                                     // uniform
+      const float r = vref / vs;
+#pragma unroll
+      for (int n = 0; n < ND; ++n) o[n] *= r;
+      vref = vs;
+    }
+    // rescale only when the maximum rose by more than 2^8 somewhere: weights stay below 2^8
+    if (__ballot(mx > m + 8.f) != 0) {
+      mx = fmaxf(mx, xor16(mx));
+      mx = fmaxf(mx, xor32(mx));
+      const float mn = fmaxf(m, mx);
+      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int n = 0; n < ND; ++n) o[n] *= al;
+    }
+    float back;
+    const float lw = value_weight(vs, vref, back) - (m == -INFINITY ? 0.f : m);
+    h8 pa[2];
+    float ls = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float p = sc[e] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sc[e] + lw);
+      ls += p;
+      pa[e >> 3][e & 7] = (_Float16)p;
+    }
+    l += ls * back;
+#pragma unroll
+    for (int n = 0; n < ND; ++n) {
+      o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h8<FP8>(vr[n].x, vr[n].y), pa[0], o[n], 0, 0, 0);
+      o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h8<FP8>(vr[n].z, vr[n].w), pa[1], o[n], 0, 0, 0);
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < mine; i += 2) {                    // the next page's loads before this one's maths
+    load_page(min(i + 1, mine - 1), kb[1], vb[1]);
+    use_page(i, kb[0], vb[0]);
+    load_page(min(i + 2, mine - 1), kb[0], vb[0]);
+    if (i + 1 < mine) use_page(i + 1, kb[1], vb[1]);
+  }
+  l += xor16(l);
+  l += xor32(l);
+
+  // merge the waves: lane (head pr, kg) holds dims 16 n + 4 kg + 0..3 of its head
+  __shared__ float wm[NW][16], wl[NW][16];
+  __shared__ __align__(16) float wo[NW][16][D + 4];
+  if (kg == 0) { wm[wave][pr] = m; wl[wave][pr] = l; }
+  if (pr < gn) {
+#pragma unroll
+    for (int n = 0; n < ND; ++n) *reinterpret_cast<f4*>(&wo[wave][pr][16 * n + 4 * kg]) = o[n] * vref;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < gn * (D / 4); i += 64 * NW) {
+    const int g = i / (D / 4), d = 4 * (i % (D / 4));
+    float M = wm[0][g];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) M = fmaxf(M, wm[w][g]);
+    float L = 0.f;
+    f4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float e = wm[w][g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wm[w][g] - M);
+      // a wave whose l is NaN saw a poisoned page: its maximum may still be -inf
+      const float lw = wl[w][g];
+      L += lw != lw ? lw : lw * e;
+      if (e != 0.f) y += *reinterpret_cast<f4*>(&wo[w][g][d]) * e;
+    }
+    const int h = kh * a.G + h0 + g;
+    if (a.parts > 1 || a.x8) {
+      const long row = ((long)part * a.sg.N + t) * a.H + h;
+      *reinterpret_cast<f4*>(a.po + row * D + d) = y;
+      if (d == 0) { a.pml[2 * row] = M; a.pml[2 * row + 1] = L; }
+    } else {
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      uint16_t* at = static_cast<uint16_t*>(a.out) + (long)t * a.so_tok + (long)h * a.so_head + d;
+      const uint32_t w0 = Elem<T>::put(y[0] * inv) | (uint32_t)Elem<T>::put(y[1] * inv) << 16;
+      const uint32_t w1 = Elem<T>::put(y[2] * inv) | (uint32_t)Elem<T>::put(y[3] * inv) << 16;
+      if (a.wide_o) {
+        *reinterpret_cast<uint2*>(at) = make_uint2(w0, w1);
+      } else {
+        at[0] = (uint16_t)w0; at[1] = (uint16_t)(w0 >> 16); at[2] = (uint16_t)w1; at[3] = (uint16_t)(w1 >> 16);
+      }
+    }
+  }
+}
+
+// Joins the partials of one (row, head): NW waves take every NW'th partial, a lane D / 64 dims.
+// DECODE: a row's number of partials follows from its position; prompt: a.parts of each row that is in
+// a segment.
+template <int D, int T, int NW, bool DECODE>
+__global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int h = blockIdx.x, t = blockIdx.y;
+  int np = a.parts;
+  if (DECODE) {
+    const int pos = a.sg.start[t];
+    np = max(1, min(np, dec_parts(seen_pages(pos, pos, a.span, a.window, a.sinks).n)));
+  } else {
+    int pos;
+    if (!find_row(a.sg, t, pos)) return;                 // no partials: the output row stays
+  }
+  const long row = (long)t * a.H + h, step = (long)a.sg.N * a.H;
+  float M = -INFINITY, L = 0.f;
+  float y[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) y[e] = 0.f;
+  for (int b = 0; b < np; b += 64) {                     // lane = partial
+    const bool in = b + lane < np;
+    const long at = row + (long)min(b + lane, np - 1) * step;
+    const float pm = in ? a.pml[2 * at] : -INFINITY, pl = in ? a.pml[2 * at + 1] : 0.f;
+    float mx = pm;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    const float mn = fmaxf(M, mx);
+    const float al = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
+    const float w = pm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(pm - mn);
+    float ls = pl != pl ? pl : pl * w;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o, 64);
+    L = L * al + ls;
+    M = mn;
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] *= al;
+    const int n = min(64, np - b);
+    constexpr int B = 8;
+    for (int i = wave; i < n; i += NW * B) {             // B partials in flight
+      float x[B][E], ww[B];
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const int p = min(i + NW * u, n - 1);
+        const float* src = a.po + (row + (long)(b + p) * step) * D + E * lane;
+        ww[u] = i + NW * u < n ? __shfl(w, p, 64) : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = src[e];
+      }
+#pragma unroll
+      for (int u = 0; u < B; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          y[e] = ww[u] != 0.f ? __fmaf_rn(ww[u], x[u][e], y[e]) : y[e];
+    }
+  }
+  if constexpr (NW > 1) {
+    __shared__ float part[NW][D];
+#pragma unroll
+    for (int e = 0; e < E; ++e) part[wave][E * lane + e] = y[e];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < NW; ++w)
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] += part[w][E * lane + e];
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int e = 0; e < E; ++e) y[e] *= inv;
+  if (a.out) {
+    uint16_t* at = static_cast<uint16_t*>(a.out) + (long)t * a.so_tok + (long)h * a.so_head + E * lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e) at[e] = Elem<T>::put(y[e]);
+  }
+  if (DECODE && a.x8) {                                  // Q8: blocks of 32 dims, sums of 16
+    const long K = (long)a.H * D, col = (long)h * D + E * lane;
+    float amax = fabsf(y[0]);
+    if (E > 1) amax = fmaxf(amax, fabsf(y[E - 1]));
+#pragma unroll
+    for (int o = 16 / E; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+    const float d = amax / 127.f;
+    int sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = d > 0.f ? (int)__builtin_rintf(y[e] / d) : 0;
+      a.x8[t * K + col + e] = (int8_t)c;
+      sum += c;
+    }
+#pragma unroll
+    for (int o = 8 / E; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if ((col & 31) == 0) a.dx[(t * K + col) >> 5] = d;
+    if ((col & 15) == 0) a.sx[(t * K + col) >> 4] = d * (float)sum;
+  }
+}
+
+// ---------------------------------------------------------------- prompt attention
+// Rows of one KV head are token-major, row = token x G + head in group; a workgroup has NW waves of 32
+// rows.  Each page goes through LDS once for all of them, turned to fp16 on the way (double buffered;
+// the next page's loads are in flight during this one's maths).  S^T = K Q^T and O^T = V^T P^T on
+// v_mfma_f32_32x32x16_f16, a lane owns one query row: softmax and rescaling need one exchange (lane
+// ^ 32).  The key of position p lies in LDS row p with bits 2 and 3 swapped, so that the score
+// registers of a lane are, in order, the P operand's consecutive positions: P never moves.
+__device__ __forceinline__ int swap23(int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); }
+
+template <int D, bool FP8, int T, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a) {
+  constexpr int NT = 64 * NW, RB = 2 * D, KT = kPage * RB, BUF = 2 * KT;    // bytes: key row, tile, K + V
+  constexpr int KC = RB / 16 - 1;                        // swizzle mask of a key row's 16-byte chunks
+  constexpr int NCH = kPage * D / 16, CH = (NCH + NT - 1) / NT;             // 16-code chunks a thread
+  constexpr int KS = D / 16, DB = D / 32;
+  __shared__ __align__(16) char lds[2 * BUF];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, hh = lane >> 5;
+  const int kh = blockIdx.x % a.c.Hkv;
+  // later pieces (of a causal prompt: the longest) first
+  const int unit = a.units - 1 - (int)(blockIdx.x / a.c.Hkv);
+  int s, piece;
+  if (!find_piece(a.sg, unit, [&](int n, int) { return (int)(((long)n * a.G + 32 * NW - 1) / (32 * NW)); }, s,
+                  piece))
+    return;
+  int row0, cnt, start;
+  a.sg.get(s, row0, cnt, start);
+  const int rows = cnt * a.G, R0 = piece * 32 * NW;
+  const int span = min(a.span, a.c.width * kPage);
+  const int t_hi = min(cnt - 1, (R0 + 32 * NW - 1) / a.G);
+  const Seen seen = seen_pages(start + R0 / a.G, start + t_hi, span, a.window, a.sinks);
+  const int each = (seen.n + a.parts - 1) / a.parts;
+  const int t0 = min(seen.n, (int)blockIdx.y * each), t1 = min(seen.n, t0 + each);
+  // this lane's row
+  const int rr = R0 + wave * 32 + r;
+  const bool valid = rr < rows;
+  const int tok = valid ? rr / a.G : cnt - 1;
+  const int head = kh * a.G + (valid ? rr - tok * a.G : 0);
+  const int pos = start + tok;
+  // this wave's positions
+  const bool wave_in = R0 + wave * 32 < rows;
+  const int w_lo = start + min(cnt - 1, (R0 + wave * 32) / a.G);
+  const int w_hi = start + min(cnt - 1, (R0 + wave * 32 + 31) / a.G);
+  const int end = min(start + cnt, span);                // keys behind it were never written
+
+  h8 qa[KS];
+  float qf = a.c2;
+  {
+    const uint16_t* qr = a.q + (long)(row0 + tok) * a.sq_tok + (long)head * a.sq_head;
+    float x[KS][8], amax = 0.f;
+#pragma unroll
+    for (int st = 0; st < KS; ++st) {
+      load_n<T, 8>(qr + 16 * st + 8 * hh, a.wide_q, x[st]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[st][e]));
+    }
+    float f = 1.f;
+    if constexpr (T == kBF16) {
+      amax = fmaxf(amax, xor32(amax));
+      f = fit_f16(amax);
+      qf /= f;
+    }
+#pragma unroll
+    for (int st = 0; st < KS; ++st)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qa[st][e] = (_Float16)(x[st][e] * f);
+  }
+  float m = -INFINITY, l = 0.f, vref = 0.f;
+  f16v o[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+
+  uint4 kr[CH], vr[CH];
+  auto load_tile = [&](int id, int base) __attribute__((always_inline)) {
+    const long at = ((long)max(id, 0) * a.c.Hkv + kh) * kPage * D;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int c = tid + u * NT;
+      if (NCH % NT == 0 || c < NCH) {
+        kr[u] = reinterpret_cast<const uint4*>(a.c.k + at)[c];
+        vr[u] = reinterpret_cast<const uint4*>(a.c.v + at)[c];
+      }
+    }
+  };
+  auto store_tile = [&](int buf, int base) __attribute__((always_inline)) {
+    char* kl = lds + buf * BUF;
+    char* vl = kl + KT;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int c = tid + u * NT;
+      if (NCH % NT == 0 || c < NCH) {
+        const int p = c / (D / 16), ch = 2 * (c % (D / 16)), row = swap23(p);
+        *reinterpret_cast<h8*>(kl + row * RB + ((ch ^ (row & KC)) << 4)) = codes_h8<FP8>(kr[u].x, kr[u].y);
+        *reinterpret_cast<h8*>(kl + row * RB + (((ch + 1) ^ (row & KC)) << 4)) = codes_h8<FP8>(kr[u].z, kr[u].w);
+        const int d = c >> 2, vch = 2 * (c & 3);
+        uint32_t w[4] = {vr[u].x, vr[u].y, vr[u].z, vr[u].w};
+        if (FP8 && base + kPage > end) {                 // codes never written may be NaN: 0 x NaN
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (base + 16 * (c & 3) + e >= end) w[e >> 2] &= ~(0xffu << (8 * (e & 3)));
+        }
+        *reinterpret_cast<h8*>(vl + d * 128 + ((vch ^ (d & 7)) << 4)) = codes_h8<FP8>(w[0], w[1]);
+        *reinterpret_cast<h8*>(vl + d * 128 + (((vch + 1) ^ (d & 7)) << 4)) = codes_h8<FP8>(w[2], w[3]);
+      }
+    }
+  };
+  auto scales = [&](int id, float& ks, float& vs) __attribute__((always_inline)) {
+    const long sc = (long)max(id, 0) * a.c.Hkv + kh;
+    ks = a.c.ks[sc];
+    vs = a.c.vs[sc];
+  };
+
+  int id = -1, id1 = -1;
+  float ks = 0.f, vs = 0.f;
+  if (t0 < t1) {
+    id = a.c.page(s, seen.page(t0));
+    load_tile(id, seen.page(t0) * kPage);
+    scales(id, ks, vs);
+    id1 = t0 + 1 < t1 ? a.c.page(s, seen.page(t0 + 1)) : -1;
+    store_tile(0, seen.page(t0) * kPage);
+  }
+  __syncthreads();
+  for (int kt = t0; kt < t1; ++kt) {
+    const int buf = (kt - t0) & 1;
+    const int base = seen.page(kt) * kPage;
+    const int next = kt + 1 < t1 ? seen.page(kt + 1) * kPage : 0;
+    float ks1 = 0.f, vs1 = 0.f;
+    int id2 = -1;
+    if (kt + 1 < t1) {
+      load_tile(id1, next);
+      scales(id1, ks1, vs1);
+      if (kt + 2 < t1) id2 = a.c.page(s, seen.page(kt + 2));
+    }
+    const bool hidden = base > w_hi || (a.window > 0 && base + kPage - 1 <= w_lo - a.window && base >= a.sinks);
+    if (wave_in && id >= 0 && !hidden) {
+      const char* kl = lds + buf * BUF;
+      const char* vl = kl + KT;
+      f16v sc[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[b][i] = 0.f;
+        const int row = 32 * b + r;
+#pragma unroll
+        for (int st = 0; st < KS; ++st) {
+          const h8 kf = *reinterpret_cast<const h8*>(kl + row * RB + (((2 * st + hh) ^ (row & KC)) << 4));
+          sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qa[st], sc[b], 0, 0, 0);
+        }
+      }
+      const float f = ks * qf;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[b][i] *= f;
+      const bool whole = base + kPage - 1 <= w_lo && base + kPage <= end &&
+                         (a.window <= 0 || base > w_hi - a.window || base + kPage <= a.sinks);
+      if (!whole) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = base + 32 * b + 16 * (i >> 3) + 8 * hh + (i & 7);
+            const bool in = j <= pos && j < end && (a.window <= 0 || j > pos - a.window || j < a.sinks);
+            sc[b][i] = in ? sc[b][i] : -INFINITY;
+          }
+      }
+      float mx = sc[0][0];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
+      if (vs > vref) {
+        const float q = vref / vs;
+#pragma unroll
+        for (int b = 0; b < DB; ++b) o[b] *= q;
+        vref = vs;
+      }
+      if (__ballot(mx > m + 8.f) != 0) {
+        mx = fmaxf(mx, xor32(mx));
+        const float mn = fmaxf(m, mx);
+        const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= al;
+#pragma unroll
+        for (int b = 0; b < DB; ++b) o[b] *= al;
+      }
+      float back;
+      const float lw = value_weight(vs, vref, back) - (m == -INFINITY ? 0.f : m);
+      h8 pa[4];
+      float ls = 0.f;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          // a NaN weight (a poisoned page) must not reach rows that do not see the key
+          const float p = !whole && sc[b][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sc[b][i] + lw);
+          ls += p;
+          pa[2 * b + (i >> 3)][i & 7] = (_Float16)p;
+        }
+      l += ls * back;
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+          const int d = 32 * b + r;
+          const h8 vf = *reinterpret_cast<const h8*>(vl + d * 128 + (((2 * st + hh) ^ (d & 7)) << 4));
+          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pa[st], o[b], 0, 0, 0);
+        }
+    }
+    if (kt + 1 < t1) store_tile(buf ^ 1, next);
+    id = id1; id1 = id2; ks = ks1; vs = vs1;
+    __syncthreads();
+  }
+  l += xor32(l);
+  if (!valid) return;
+  const long grow = (long)row0 + tok;
+  if (a.parts > 1) {
+    const long prow = ((long)blockIdx.y * a.sg.N + grow) * a.H + head;
+    float* at = a.po + prow * D;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<f4*>(at + 32 * b + 2 * i + 4 * hh) =
+            f4{o[b][i] * vref, o[b][i + 1] * vref, o[b][i + 2] * vref, o[b][i + 3] * vref};
+    if (hh == 0) { a.pml[2 * prow] = m; a.pml[2 * prow + 1] = l; }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : vref / l;
+  uint16_t* at = static_cast<uint16_t*>(a.out) + grow * a.so_tok + (long)head * a.so_head;
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      uint16_t* w = at + 32 * b + 2 * i + 4 * hh;
+      const uint32_t w0 = Elem<T>::put(o[b][i] * inv) | (uint32_t)Elem<T>::put(o[b][i + 1] * inv) << 16;
+      const uint32_t w1 = Elem<T>::put(o[b][i + 2] * inv) | (uint32_t)Elem<T>::put(o[b][i + 3] * inv) << 16;
+      if (a.wide_o) {
+        *reinterpret_cast<uint2*>(w) = make_uint2(w0, w1);
+      } else {
+        w[0] = (uint16_t)w0; w[1] = (uint16_t)(w0 >> 16); w[2] = (uint16_t)w1; w[3] = (uint16_t)(w1 >> 16);
+      }
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int amdk8s_llm_kv8_page() { return kPage; }
+
+}  // extern "C"
+
+namespace {
+
+bool wide16(const void* p, long esize, long s0, long s1) {
+  return ((uintptr_t)p & 15) == 0 && (s0 * esize) % 16 == 0 && (s1 * esize) % 16 == 0;
+}
+int launched() { return hipGetLastError() == hipSuccess ? 0 : 1; }
+
+// D and the code type to template arguments
+template <typename F>
+int by_format(int D, int fp8, F f) {
+  using I64 = std::integral_constant<int, 64>;
+  using I128 = std::integral_constant<int, 128>;
+  if (D == 128) return fp8 ? f(I128{}, std::true_type{}) : f(I128{}, std::false_type{});
+  if (D == 64) return fp8 ? f(I64{}, std::true_type{}) : f(I64{}, std::false_type{});
+  return 2;
+}
+
+Pool make_pool(void* k, void* v, void* ks, void* vs, const void* table, int pool, int Hkv, int width, int stride) {
+  return Pool{static_cast<uint8_t*>(k), static_cast<uint8_t*>(v), static_cast<float*>(ks), static_cast<float*>(vs),
+              static_cast<const int*>(table), pool, Hkv, width, stride};
+}
+bool bad_pool(const void* k, const void* v, const void* ks, const void* vs, const void* table, int pool, int Hkv,
+              int width) {
+  return !k || !v || !ks || !vs || !table || pool < 1 || Hkv < 1 || width < 1 || width > (1 << 24) ||
+         (((uintptr_t)k | (uintptr_t)v) & 15);
+}
+
+}  // namespace
+
+extern "C" {
+
+// rc: 0 launched, 1 launch error, 2 bad argument.
+// Rows of k / v (and q) of S segments into the cache; cos_t null: no rotation; q null: keys only.
+// type: element type of k, v, q (0 fp16, 1 bf16, 2 fp32); otype: of qo (0, 1).
+int amdk8s_llm_kv8_append(void* kc, void* vc, void* ks, void* vs, const void* table, int pool, int Hkv, int D,
+                          int fp8, int width, int tstride, const void* start, const void* cu, int S, int N,
+                          const void* k, long sk_tok, long sk_head, const void* v, long sv_tok, long sv_head,
+                          const void* q, long sq_tok, long sq_head, void* qo, long so_tok, long so_head, int H,
+                          const void* cos_t, const void* sin_t, int table_rows, int type, int otype, void* stream) {
+  if (bad_pool(kc, vc, ks, vs, table, pool, Hkv, width) || !start || !cu || S < 1 || N < 1 || !k || !v) return 2;
+  if ((q != nullptr) != (qo != nullptr) || (q && H < 1) || (cos_t != nullptr) != (sin_t != nullptr)) return 2;
+  if (type < 0 || type > 2 || otype < 0 || otype > 1 || (type < 2 && otype != type)) return 2;
+  if (cos_t && (table_rows < width * (long)kPage || (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15))) return 2;
+  AppendArgs a{};
+  a.c = make_pool(kc, vc, ks, vs, table, pool, Hkv, width, tstride);
+  a.sg = Segs{static_cast<const int*>(start), static_cast<const int*>(cu), S, N};
+  a.k = k; a.v = v; a.q = q; a.qo = qo;
+  a.cos_t = static_cast<const float*>(cos_t);
+  a.sin_t = static_cast<const float*>(sin_t);
+  a.sk_tok = sk_tok; a.sk_head = sk_head; a.sv_tok = sv_tok; a.sv_head = sv_head;
+  a.sq_tok = sq_tok; a.sq_head = sq_head; a.so_tok = so_tok; a.so_head = so_head;
+  a.H = H;
+  const int es = type == kF32 ? 4 : 2;
+  a.wide_kv = wide16(k, es, sk_tok, sk_head) && wide16(v, es, sv_tok, sv_head);
+  a.wide_q = q && wide16(q, es, sq_tok, sq_head) && wide16(qo, 2, so_tok, so_head);
+  a.table_rows = cos_t ? table_rows : 0x7fffffff;
+  const long units = most_pages(N, S), qb = q ? (N + 3L) / 4 : 0;
+  if (units * Hkv + qb > 0x7fffffffL) return 2;
+  a.units = (int)units;
+  const dim3 grid((unsigned)(units * Hkv + qb));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return by_format(D, fp8, [&](auto d, auto f) -> int {
+    constexpr int DD = decltype(d)::value;
+    constexpr bool F8 = decltype(f)::value;
+    if (type == kF16) hipLaunchKernelGGL((kv8_append_kernel<DD, F8, kF16, kF16>), grid, dim3(256), 0, st, a);
+    else if (type == kBF16) hipLaunchKernelGGL((kv8_append_kernel<DD, F8, kBF16, kBF16>), grid, dim3(256), 0, st, a);
+    else if (otype == kF16) hipLaunchKernelGGL((kv8_append_kernel<DD, F8, kF32, kF16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv8_append_kernel<DD, F8, kF32, kBF16>), grid, dim3(256), 0, st, a);
+    return launched();
+  });
+}
+
+// Cached positions of S segments as values: rows of ko / vo (type 0 fp16, 1 bf16, 2 fp32).
+int amdk8s_llm_kv8_read(const void* kc, const void* vc, const void* ks, const void* vs, const void* table, int pool,
+                        int Hkv, int D, int fp8, int width, int tstride, const void* start, const void* cu, int S,
+                        int N, void* ko, long sk_tok, long sk_head, void* vo, long sv_tok, long sv_head, int type,
+                        void* stream) {
+  if (bad_pool(kc, vc, ks, vs, table, pool, Hkv, width) || !start || !cu || S < 1 || N < 1 || !ko || !vo) return 2;
+  if (type < 0 || type > 2) return 2;
+  ReadArgs a{};
+  a.c = make_pool(const_cast<void*>(kc), const_cast<void*>(vc), const_cast<void*>(ks), const_cast<void*>(vs), table,
+                  pool, Hkv, width, tstride);
+  a.sg = Segs{static_cast<const int*>(start), static_cast<const int*>(cu), S, N};
+  a.ko = ko; a.vo = vo;
+  a.sk_tok = sk_tok; a.sk_head = sk_head; a.sv_tok = sv_tok; a.sv_head = sv_head;
+  const int es = type == kF32 ? 4 : 2;
+  a.wide = wide16(ko, es, sk_tok, sk_head) && wide16(vo, es, sv_tok, sv_head);
+  const long blocks = most_pages(N, S) * Hkv;
+  if (blocks > 0x7fffffffL) return 2;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)blocks);
+  return by_format(D, fp8, [&](auto d, auto f) -> int {
+    constexpr int DD = decltype(d)::value;
+    constexpr bool F8 = decltype(f)::value;
+    if (type == kF16) hipLaunchKernelGGL((kv8_read_kernel<DD, F8, kF16>), grid, dim3(256), 0, st, a);
+    else if (type == kBF16) hipLaunchKernelGGL((kv8_read_kernel<DD, F8, kBF16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv8_read_kernel<DD, F8, kF32>), grid, dim3(256), 0, st, a);
+    return launched();
+  });
+}
+
+// fp32 workspace (in floats) of a decode call: 0 when its partials need no join
+long amdk8s_llm_kv8_decode_work(int S, int H, int D, int span, int window, int sinks, int q8) {
+  if (S < 1 || H < 1 || D < 1 || span < 1 || window < 0 || sinks < 0) return -1;
+  // the most pages any position sees: the window's (its two ends may be cut) and the sinks'
+  long n = (span + (long)kPage - 1) / kPage;
+  if (window > 0) {
+    const long w = (window + 62L) / kPage + 1 + (sinks + 63L) / kPage;
+    n = w < n ? w : n;
+  }
+  const long parts = dec_parts_most((int)n);
+  return parts == 1 && !q8 ? 0 : parts * S * H * (D + 2);
+}
+
+// One query row a sequence at position pos[s] (-1: nothing to see, zeros).  span: keys at or behind it are
+// not attended.  type: q and out (0 fp16, 1 bf16).  x8 / dx / sx (nullable): the output as Q8 rows; out
+// may then be null.
+int amdk8s_llm_kv8_decode(const void* kc, const void* vc, const void* ks, const void* vs, const void* table,
+                          int pool, int Hkv, int D, int fp8, int width, int tstride, const void* q, long sq_tok,
+                          long sq_head, const void* pos, int S, int H, int span, int window, int sinks, float scale,
+                          void* out, long so_tok, long so_head, int type, void* x8, void* dx, void* sx, void* work,
+                          long work_floats, void* stream) {
+  if (bad_pool(kc, vc, ks, vs, table, pool, Hkv, width) || !q || !pos || S < 1 || S > 65535 || H < 1 || H % Hkv)
+    return 2;
+  if (type < 0 || type > 1 || span < 1 || span > width * (long)kPage || window < 0 || window > (1 << 30) ||
+      sinks < 0 || sinks > (1 << 30))
+    return 2;
+  if ((!out && !x8) || (x8 && (!dx || !sx))) return 2;
+  const long need = amdk8s_llm_kv8_decode_work(S, H, D, span, window, sinks, x8 != nullptr);
+  if (need > work_floats || (need && (!work || ((uintptr_t)work & 15)))) return 2;
+  const long parts = need ? need / ((long)S * H * (D + 2)) : 1;
+  const long gx = (long)Hkv * ((H / Hkv + 15) / 16);
+  if (parts > 65535) return 2;
+  AttnArgs a{};
+  a.c = make_pool(const_cast<void*>(kc), const_cast<void*>(vc), const_cast<void*>(ks), const_cast<void*>(vs), table,
+                  pool, Hkv, width, tstride);
+  a.sg = Segs{static_cast<const int*>(pos), nullptr, S, S};
+  a.q = static_cast<const uint16_t*>(q);
+  a.out = out;
+  a.po = static_cast<float*>(work);
+  a.pml = need ? a.po + parts * S * H * D : nullptr;
+  a.x8 = static_cast<int8_t*>(x8);
+  a.dx = static_cast<float*>(dx);
+  a.sx = static_cast<float*>(sx);
+  a.sq_tok = sq_tok; a.sq_head = sq_head; a.so_tok = so_tok; a.so_head = so_head;
+  a.H = H; a.G = H / Hkv; a.span = span; a.window = window; a.sinks = sinks; a.parts = (int)parts;
+  a.c2 = scale * 1.4426950408889634f;
+  a.wide_q = wide16(q, 2, sq_tok, sq_head);
+  a.wide_o = out && wide16(out, 2, so_tok, so_head);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)gx, (unsigned)parts, S);
+  return by_format(D, fp8, [&](auto d, auto f) -> int {
+    constexpr int DD = decltype(d)::value;
+    constexpr bool F8 = decltype(f)::value;
+    if (type == kF16) hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kF16>), grid, dim3(64 * kDecWaves), 0, st, a);
+    else hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kBF16>), grid, dim3(64 * kDecWaves), 0, st, a);
+    if (need) {
+      if (type == kF16) hipLaunchKernelGGL((kv8_join_kernel<DD, kF16, 4, true>), dim3(H, S), dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((kv8_join_kernel<DD, kBF16, 4, true>), dim3(H, S), dim3(256), 0, st, a);
+    }
+    return launched();
+  });
+}
+
+}  // extern "C"
+
+namespace {
+
+constexpr int kPromptWaves = 4;
+constexpr int kPromptGrid = 512;                         // two workgroups on each of the 256 CUs
+
+// workgroups that share a row block's keys: as many as fill the chip when there are few row blocks, each
+// with at least 8 pages
+int prompt_parts(long N, int S, int H, int Hkv, int span, int window, int sinks, long& units) {
+  const int rows = 32 * kPromptWaves, G = H / Hkv;
+  units = N * G / rows + S;
+  if (G <= rows && units > N) units = N;
+  long n = (span + (long)kPage - 1) / kPage;
+  if (window > 0) {
+    const long w = (window + (rows + G - 1) / G + 62L) / kPage + 1 + (sinks + 63L) / kPage;
+    n = w < n ? w : n;
+  }
+  long parts = kPromptGrid / (units * Hkv);
+  if (parts > n / 8) parts = n / 8;
+  return parts < 1 ? 1 : (int)parts;
+}
+
+}  // namespace
+
+extern "C" {
+
+// fp32 workspace (in floats) of a prompt call
+long amdk8s_llm_kv8_prompt_work(int N, int S, int H, int Hkv, int D, int span, int window, int sinks) {
+  if (N < 1 || S < 1 || Hkv < 1 || H < Hkv || H % Hkv || D < 1 || span < 1 || window < 0 || sinks < 0) return -1;
+  long units;
+  const long parts = prompt_parts(N, S, H, Hkv, span, window, sinks, units);
+  return parts == 1 ? 0 : parts * N * H * (D + 2);
+}
+
+// Query rows of S segments (row cu[s] + i at position start[s] + i) over the cache, their own keys
+// included; rows in no segment are left as they are.
+int amdk8s_llm_kv8_prompt(const void* kc, const void* vc, const void* ks, const void* vs, const void* table,
+                          int pool, int Hkv, int D, int fp8, int width, int tstride, const void* start,
+                          const void* cu, int S, int N, const void* q, long sq_tok, long sq_head, int H, int span,
+                          int window, int sinks, float scale, void* out, long so_tok, long so_head, int type,
+                          void* work, long work_floats, void* stream) {
+  if (bad_pool(kc, vc, ks, vs, table, pool, Hkv, width) || !q || !out || !start || !cu || S < 1 || N < 1 || H < 1 ||
+      H % Hkv)
+    return 2;
+  if (type < 0 || type > 1 || span < 1 || span > width * (long)kPage || window < 0 || window > (1 << 30) ||
+      sinks < 0 || sinks > (1 << 30) || (long)N * (H / Hkv) > 0x3fffffffL)
+    return 2;
+  long units;
+  const long parts = prompt_parts(N, S, H, Hkv, span, window, sinks, units);
+  const long need = parts == 1 ? 0 : parts * N * H * (D + 2);
+  if (need > work_floats || (need && (!work || ((uintptr_t)work & 15)))) return 2;
+  if (units * Hkv > 0x7fffffffL || parts > 65535 || (parts > 1 && N > 65535)) return 2;
+  AttnArgs a{};
+  a.c = make_pool(const_cast<void*>(kc), const_cast<void*>(vc), const_cast<void*>(ks), const_cast<void*>(vs), table,
+                  pool, Hkv, width, tstride);
+  a.sg = Segs{static_cast<const int*>(start), static_cast<const int*>(cu), S, N};
+  a.q = static_cast<const uint16_t*>(q);
+  a.out = out;
+  a.po = static_cast<float*>(work);
+  a.pml = need ? a.po + parts * N * H * D : nullptr;
+  a.sq_tok = sq_tok; a.sq_head = sq_head; a.so_tok = so_tok; a.so_head = so_head;
+  a.H = H; a.G = H / Hkv; a.span = span; a.window = window; a.sinks = sinks; a.parts = (int)parts;
+  a.units = (int)units;
+  a.c2 = scale * 1.4426950408889634f;
+  a.wide_q = wide16(q, 2, sq_tok, sq_head);
+  a.wide_o = wide16(out, 2, so_tok, so_head);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(units * Hkv), (unsigned)parts);
+  return by_format(D, fp8, [&](auto d, auto f) -> int {
+    constexpr int DD = decltype(d)::value;
+    constexpr bool F8 = decltype(f)::value;
+    constexpr int NW = kPromptWaves;
+    if (type == kF16) hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kF16, NW>), grid, dim3(64 * NW), 0, st, a);
+    else hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kBF16, NW>), grid, dim3(64 * NW), 0, st, a);
+    if (need) {
+      if (type == kF16) hipLaunchKernelGGL((kv8_join_kernel<DD, kF16, 1, false>), dim3(H, N), dim3(64), 0, st, a);
+      else hipLaunchKernelGGL((kv8_join_kernel<DD, kBF16, 1, false>), dim3(H, N), dim3(64), 0, st, a);
+    }
+    return launched();
+  });
+}
+
+}  // extern "C"
