@@ -173,16 +173,19 @@ struct Segs {
   }
 };
 
-// The unit'th piece of all segments, each cut into pieces by `count` (pieces of segment s); the whole
+// A piece of a segment: the segment, its rows (row .. row + cnt - 1, at pos ..) and the piece's index.
+struct Piece {
+  int s, index, row, cnt, pos;
+};
+// The unit'th piece of all segments, each cut into pieces by `count` (pieces of n rows at pos); the whole
 // wave calls it and gets the same answer.  False: there are fewer pieces.
 template <typename F>
-__device__ __forceinline__ bool find_piece(const Segs& sg, int unit, F count, int& s, int& piece) {
+__device__ __forceinline__ bool find_piece(const Segs& sg, int unit, F count, Piece& out) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int base = 0; base < sg.S; base += 64) {
-    int c = 0;
+    int c = 0, row = 0, n = 0, pos = 0;
     if (base + lane < sg.S) {
-      int row, n, pos;
       sg.get(base + lane, row, n, pos);
       c = n > 0 ? count(n, pos) : 0;
     }
@@ -195,11 +198,14 @@ __device__ __forceinline__ bool find_piece(const Segs& sg, int unit, F count, in
     const uint64_t past = __ballot(before + inc > unit);
     if (past) {
       const int hit = __builtin_ctzll(past);
-      s = __builtin_amdgcn_readfirstlane(base + hit);
-      piece = __builtin_amdgcn_readfirstlane(unit - before - (__shfl(inc, hit, 64) - __shfl(c, hit, 64)));
+      out.s = base + hit;
+      out.index = unit - before - (__builtin_amdgcn_readlane(inc, hit) - __builtin_amdgcn_readlane(c, hit));
+      out.row = __builtin_amdgcn_readlane(row, hit);
+      out.cnt = __builtin_amdgcn_readlane(n, hit);
+      out.pos = __builtin_amdgcn_readlane(pos, hit);
       return true;
     }
-    before += __shfl(inc, 63, 64);
+    before += __builtin_amdgcn_readlane(inc, 63);
   }
   return false;
 }
@@ -323,12 +329,11 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
   __shared__ uint32_t red[2][4];
   __shared__ __align__(16) uint8_t img[kPage][D + 16];   // value codes by position
   const int kh = blockIdx.x % a.c.Hkv;
-  int s, piece;
-  if (!find_piece(a.sg, blockIdx.x / a.c.Hkv, [](int n, int p) { return pages_of(n, p); }, s, piece)) return;
-  int row, cnt, pos;
-  a.sg.get(s, row, cnt, pos);
-  const int j = pos / kPage + piece;
-  const int id = a.c.page(s, j);
+  Piece pc;
+  if (!find_piece(a.sg, blockIdx.x / a.c.Hkv, [](int n, int p) { return pages_of(n, p); }, pc)) return;
+  const int pos = pc.pos, cnt = pc.cnt, row = pc.row;
+  const int j = pos / kPage + pc.index;
+  const int id = a.c.page(pc.s, j);
   if (id < 0) return;
   const int r0 = max(pos - j * kPage, 0), r1 = min(pos + cnt - j * kPage, kPage);   // new rows
   const long n0 = (long)row + j * kPage - pos;           // input row of the page's position 0
@@ -449,14 +454,13 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
   __shared__ __align__(16) uint8_t img[kPage][D + 16];
   const int tid = threadIdx.x;
   const int kh = blockIdx.x % a.c.Hkv;
-  int s, piece;
-  if (!find_piece(a.sg, blockIdx.x / a.c.Hkv, [](int n, int p) { return pages_of(n, p); }, s, piece)) return;
-  int row, cnt, pos;
-  a.sg.get(s, row, cnt, pos);
-  const int j = pos / kPage + piece;
+  Piece pc;
+  if (!find_piece(a.sg, blockIdx.x / a.c.Hkv, [](int n, int p) { return pages_of(n, p); }, pc)) return;
+  const int pos = pc.pos, cnt = pc.cnt, row = pc.row;
+  const int j = pos / kPage + pc.index;
   const int r0 = max(pos - j * kPage, 0), r1 = min(pos + cnt - j * kPage, kPage);
   const long n0 = (long)row + j * kPage - pos;
-  const int id = a.c.page(s, j);
+  const int id = a.c.page(pc.s, j);
   const bool live = id >= 0;
   const long sc = (long)max(id, 0) * a.c.Hkv + kh;
   const uint8_t* kc = a.c.k + sc * kPage * D;
@@ -559,82 +563,64 @@ struct AttnArgs {
   float* sx;
   long sq_tok, sq_head, so_tok, so_head;
   int H, G, span, window, sinks, parts, units;
+  int per;                 // decode: pages a wave (at most 64)
   float c2;                // scale x log2(e)
   bool wide_q, wide_o;
 };
 
-// pages a workgroup streams, and workgroups (partials) of a token that sees n pages: its own count
-// decides, so that its bits do not depend on the batch
-constexpr int kDecWaves = 4;
-constexpr int kDecParts = 64;
-constexpr int kDecMaxPer = 64;                           // pages a wave (a lane holds one page's table entry)
-__host__ __device__ __forceinline__ int dec_per_wave(int n) {
-  int p = 1;
-  while (p < kDecMaxPer && n > kDecParts * kDecWaves * p) p <<= 1;
-  return p;
-}
-__host__ __device__ __forceinline__ int dec_parts(int n) {
-  const int w = kDecWaves * dec_per_wave(n);
-  return (n + w - 1) / w;
-}
-inline int dec_parts_most(int n) {                       // of any count <= n
-  int m = dec_parts(n);
-  for (int e = kDecParts * kDecWaves; e < n; e <<= 1) {
-    const int p = dec_parts(e);
-    if (p > m) m = p;
-  }
-  return m;
-}
-
-// Single-token attention.  Grid (Hkv x groups of 16 heads, parts, S); a wave streams whole pages with
-// its own online softmax, no LDS and no barrier until the waves merge.  Both products on
-// v_mfma_f32_16x16x32_f16, operands straight from memory:
+// Single-token attention.  Grid (Hkv x groups of 16 heads, parts, S); workgroup part p streams pages
+// p NW per .. of the row's list, each wave whole pages with its own online softmax, no LDS and no barrier
+// until the waves merge.  Both products on v_mfma_f32_16x16x32_f16, operands straight from memory:
 // * S = K q^T: tile t of four has the rows m = 0..15 at positions 16 (m >> 2) + 4 t + (m & 3), so that
 //   lane (head pr, group kg) gets the scores of positions 16 kg .. 16 kg + 15 over the four tiles;
 // * O^T = V^T P^T: the value codes lie dim-major, a lane's 16 bytes are positions 16 kg .. + 15 of one
 //   dim: the same positions as its scores, so neither P nor V moves between lanes.  The running
 //   maximum, sum and rescaling are one head's, a lane's own.
-template <int D, bool FP8, int T>
-__global__ void __launch_bounds__(64 * kDecWaves) kv8_decode_kernel(const AttnArgs a) {
-  constexpr int NW = kDecWaves, KH = D / 64, ND = D / 16;
+// A page's keys are loaded as soon as the last page's have been used, and its values likewise: 16 KB in
+// flight a wave most of the time at half the registers of two buffers.
+template <int D, bool FP8, int T, int NW>
+__global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a) {
+  constexpr int KH = D / 64, ND = D / 16;
   const int hg = (a.G + 15) / 16;
   const int kh = blockIdx.x / hg, h0 = (blockIdx.x % hg) * 16;
   const int part = blockIdx.y, t = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pr = lane & 15, kg = lane >> 4;
   const int gn = min(16, a.G - h0);                      // heads of this workgroup
+  const int p0 = part * a.per * NW;
   const int pos = a.sg.start[t];
-  const Seen seen = seen_pages(pos, pos, a.span, a.window, a.sinks);
-  const int per = dec_per_wave(seen.n);
-  const int p0 = part * per * NW;
-  if (p0 >= seen.n && part > 0) return;                  // part 0 of an empty row writes its zeros
-  const int mine = max(0, min(per, (seen.n - p0 - wave + NW - 1) / NW));   // pages p0 + wave + NW i
-
-  // lane i: table entry and scales of this wave's i'th page
+  // lane i: table entry and scales of this wave's i'th page (pages p0 + wave + NW i of the list).
+  // Without a window the list is the table itself: its entry does not wait for the position.
   int my_id = -1;
+  if (a.window <= 0 && lane < a.per) my_id = a.c.page(t, p0 + wave + NW * lane);
+  const Seen seen = seen_pages(pos, pos, a.span, a.window, a.sinks);
+  const int mine = max(0, min(a.per, (seen.n - p0 - wave + NW - 1) / NW));
+  if (a.window > 0 && lane < mine) my_id = a.c.page(t, seen.page(p0 + wave + NW * lane));
   float my_ks = 0.f, my_vs = 0.f;
-  if (lane < mine) {
-    my_id = a.c.page(t, seen.page(p0 + wave + NW * lane));
-    if (my_id >= 0) {
-      const long sc = (long)my_id * a.c.Hkv + kh;
-      my_ks = a.c.ks[sc];
-      my_vs = a.c.vs[sc];
-    }
+  if (lane < mine && my_id >= 0) {
+    const long sc = (long)my_id * a.c.Hkv + kh;
+    my_ks = a.c.ks[sc];
+    my_vs = a.c.vs[sc];
   }
-  uint4 kb[2][4 * KH], vb[2][ND];
-  auto load_page = [&](int i, uint4 (&kr)[4 * KH], uint4 (&vr)[ND]) __attribute__((always_inline)) {
-    const int id = max(__builtin_amdgcn_readlane(my_id, i), 0);
-    const long base = ((long)id * a.c.Hkv + kh) * kPage * D;
-    const uint8_t* kp = a.c.k + base + (16 * (pr >> 2) + (pr & 3)) * D + 16 * kg;
-    const uint8_t* vp = a.c.v + base + pr * kPage + 16 * kg;
+  uint4 kr[4 * KH], vr[ND];
+  auto load_keys = [&](int i) __attribute__((always_inline)) {
+    const long id = max(__builtin_amdgcn_readlane(my_id, i), 0);
+    const uint8_t* kp = a.c.k + (id * a.c.Hkv + kh) * (kPage * D) + (16 * (pr >> 2) + (pr & 3)) * D + 16 * kg;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int h = 0; h < KH; ++h) kr[u * KH + h] = *reinterpret_cast<const uint4*>(kp + 4 * u * D + 64 * h);
+  };
+  auto load_values = [&](int i) __attribute__((always_inline)) {
+    const long id = max(__builtin_amdgcn_readlane(my_id, i), 0);
+    const uint8_t* vp = a.c.v + (id * a.c.Hkv + kh) * (kPage * D) + pr * kPage + 16 * kg;
 #pragma unroll
     for (int n = 0; n < ND; ++n) vr[n] = *reinterpret_cast<const uint4*>(vp + 16 * n * kPage);
   };
-  if (mine > 0) load_page(0, kb[0], vb[0]);
+  if (mine > 0) {
+    load_keys(0);
+    load_values(0);
+  }
 
   // q operand: head pr, dims 64 h + 16 kg + 8 u + 0..7 (the order in which the key bytes lie)
   h8 qa[2 * KH];
@@ -668,8 +654,11 @@ __global__ void __launch_bounds__(64 * kDecWaves) kv8_decode_kernel(const AttnAr
 #pragma unroll
   for (int n = 0; n < ND; ++n) o[n] = f4{0.f, 0.f, 0.f, 0.f};
 
-  auto use_page = [&](int i, uint4 (&kr)[4 * KH], uint4 (&vr)[ND]) __attribute__((always_inline)) {
-    if (__builtin_amdgcn_readlane(my_id, i) < 0) return;
+  const int last = min(pos, a.span - 1);
+#pragma unroll 1
+  for (int i = 0; i < mine; ++i) {
+    const bool more = i + 1 < mine;
+    const bool mapped = __builtin_amdgcn_readlane(my_id, i) >= 0;
     const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_ks), i));
     const float vs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_vs), i));
     const int base = seen.page(p0 + wave + NW * i) * kPage;
@@ -684,11 +673,15 @@ __global__ void __launch_bounds__(64 * kDecWaves) kv8_decode_kernel(const AttnAr
         acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h8<FP8>(w.z, w.w), qa[2 * h + 1], acc[u], 0, 0, 0);
       }
     }
+    if (more) load_keys(i + 1);
+    if (!mapped) {                                       // (uniform)
+      if (more) load_values(i + 1);
+      continue;
+    }
     const float f = ks * qf;
     float sc[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) sc[e] = acc[e >> 2][e & 3] * f;
-    const int last = min(pos, a.span - 1);
     const bool whole = base + kPage - 1 <= last &&
                        (a.window <= 0 || base > pos - a.window || base + kPage <= a.sinks);
     if (!whole) {                                        // a border inside the page (wave-uniform)
@@ -741,13 +734,7 @@ __global__ void __launch_bounds__(64 * kDecWaves) kv8_decode_kernel(const AttnAr
       o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h8<FP8>(vr[n].x, vr[n].y), pa[0], o[n], 0, 0, 0);
       o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h8<FP8>(vr[n].z, vr[n].w), pa[1], o[n], 0, 0, 0);
     }
-  };
-#pragma unroll 1
-  for (int i = 0; i < mine; i += 2) {                    // the next page's loads before this one's maths
-    load_page(min(i + 1, mine - 1), kb[1], vb[1]);
-    use_page(i, kb[0], vb[0]);
-    load_page(min(i + 2, mine - 1), kb[0], vb[0]);
-    if (i + 1 < mine) use_page(i + 1, kb[1], vb[1]);
+    if (more) load_values(i + 1);
   }
   l += xor16(l);
   l += xor32(l);
@@ -795,19 +782,15 @@ __global__ void __launch_bounds__(64 * kDecWaves) kv8_decode_kernel(const AttnAr
   }
 }
 
-// Joins the partials of one (row, head): NW waves take every NW'th partial, a lane D / 64 dims.
-// DECODE: a row's number of partials follows from its position; prompt: a.parts of each row that is in
-// a segment.
+// Joins the partials of one (row, head): NW waves take every NW'th partial, a lane D / 64 dims.  Every
+// partial's maximum and sum are written, also an empty one's (-inf, 0), whose output is not: all loads
+// go out at once and an empty one's weight is 0.
 template <int D, int T, int NW, bool DECODE>
 __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int h = blockIdx.x, t = blockIdx.y;
-  int np = a.parts;
-  if (DECODE) {
-    const int pos = a.sg.start[t];
-    np = max(1, min(np, dec_parts(seen_pages(pos, pos, a.span, a.window, a.sinks).n)));
-  } else {
+  constexpr int E = D / 64, B = 8;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = blockIdx.x, t = blockIdx.y, np = a.parts;
+  if (!DECODE) {
     int pos;
     if (!find_row(a.sg, t, pos)) return;                 // no partials: the output row stays
   }
@@ -817,9 +800,20 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
 #pragma unroll
   for (int e = 0; e < E; ++e) y[e] = 0.f;
   for (int b = 0; b < np; b += 64) {                     // lane = partial
-    const bool in = b + lane < np;
-    const long at = row + (long)min(b + lane, np - 1) * step;
-    const float pm = in ? a.pml[2 * at] : -INFINITY, pl = in ? a.pml[2 * at + 1] : 0.f;
+    const int n = min(64, np - b);
+    float x[B][E];
+    auto load = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const float* src = a.po + (row + (long)(b + min(i + NW * u, n - 1)) * step) * D + E * lane;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = src[e];
+      }
+    };
+    const long at = row + (long)(b + min(lane, n - 1)) * step;
+    float pm = a.pml[2 * at], pl = a.pml[2 * at + 1];
+    load(wave);
+    if (lane >= n) { pm = -INFINITY; pl = 0.f; }
     float mx = pm;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
@@ -833,23 +827,15 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
     M = mn;
 #pragma unroll
     for (int e = 0; e < E; ++e) y[e] *= al;
-    const int n = min(64, np - b);
-    constexpr int B = 8;
     for (int i = wave; i < n; i += NW * B) {             // B partials in flight
-      float x[B][E], ww[B];
+      if (i != wave) load(i);
 #pragma unroll
       for (int u = 0; u < B; ++u) {
         const int p = min(i + NW * u, n - 1);
-        const float* src = a.po + (row + (long)(b + p) * step) * D + E * lane;
-        ww[u] = i + NW * u < n ? __shfl(w, p, 64) : 0.f;
+        const float ww = i + NW * u < n ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), p)) : 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[u][e] = src[e];
+        for (int e = 0; e < E; ++e) y[e] = ww != 0.f ? __fmaf_rn(ww, x[u][e], y[e]) : y[e];
       }
-#pragma unroll
-      for (int u = 0; u < B; ++u)
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          y[e] = ww[u] != 0.f ? __fmaf_rn(ww[u], x[u][e], y[e]) : y[e];
     }
   }
   if constexpr (NW > 1) {
@@ -913,13 +899,11 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
   const int kh = blockIdx.x % a.c.Hkv;
   // later pieces (of a causal prompt: the longest) first
   const int unit = a.units - 1 - (int)(blockIdx.x / a.c.Hkv);
-  int s, piece;
-  if (!find_piece(a.sg, unit, [&](int n, int) { return (int)(((long)n * a.G + 32 * NW - 1) / (32 * NW)); }, s,
-                  piece))
+  Piece pc;
+  if (!find_piece(a.sg, unit, [&](int n, int) { return (int)(((long)n * a.G + 32 * NW - 1) / (32 * NW)); }, pc))
     return;
-  int row0, cnt, start;
-  a.sg.get(s, row0, cnt, start);
-  const int rows = cnt * a.G, R0 = piece * 32 * NW;
+  const int s = pc.s, row0 = pc.row, cnt = pc.cnt, start = pc.pos;
+  const int rows = cnt * a.G, R0 = pc.index * 32 * NW;
   const int span = min(a.span, a.c.width * kPage);
   const int t_hi = min(cnt - 1, (R0 + 32 * NW - 1) / a.G);
   const Seen seen = seen_pages(start + R0 / a.G, start + t_hi, span, a.window, a.sinks);
@@ -1248,16 +1232,39 @@ int amdk8s_llm_kv8_read(const void* kc, const void* vc, const void* ks, const vo
   });
 }
 
-// fp32 workspace (in floats) of a decode call: 0 when its partials need no join
-long amdk8s_llm_kv8_decode_work(int S, int H, int D, int span, int window, int sinks, int q8) {
-  if (S < 1 || H < 1 || D < 1 || span < 1 || window < 0 || sinks < 0) return -1;
-  // the most pages any position sees: the window's (its two ends may be cut) and the sinks'
-  long n = (span + (long)kPage - 1) / kPage;
+}  // extern "C"
+
+namespace {
+
+constexpr long kDecodeGrid = 768;                        // workgroups: three on each of the 256 CUs
+
+struct DecodePlan {
+  int nw, per, parts;
+};
+// Pages a wave: one until the workgroups fill the chip three deep, then as many as keep it so (a longer
+// chain of pages pays a workgroup's start and its partial output once).  Up to 8 pages run in one
+// workgroup of 8 waves, which needs no join.
+DecodePlan decode_plan(long S, int H, int Hkv, int span, int window, int sinks) {
+  long n = (span + (long)kPage - 1) / kPage;             // pages a row sees at most
   if (window > 0) {
     const long w = (window + 62L) / kPage + 1 + (sinks + 63L) / kPage;
     n = w < n ? w : n;
   }
-  const long parts = dec_parts_most((int)n);
+  if (n <= 8) return {8, 1, 1};
+  const long chains = S * Hkv * ((H / Hkv + 15) / 16);
+  long per = chains * n / (4 * kDecodeGrid);
+  per = per < 1 ? 1 : per > 64 ? 64 : per;
+  return {4, (int)per, (int)((n + 4 * per - 1) / (4 * per))};
+}
+
+}  // namespace
+
+extern "C" {
+
+// fp32 workspace (in floats) of a decode call: 0 when its partials need no join
+long amdk8s_llm_kv8_decode_work(int S, int H, int Hkv, int D, int span, int window, int sinks, int q8) {
+  if (S < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || span < 1 || window < 0 || sinks < 0) return -1;
+  const long parts = decode_plan(S, H, Hkv, span, window, sinks).parts;
   return parts == 1 && !q8 ? 0 : parts * S * H * (D + 2);
 }
 
@@ -1275,9 +1282,10 @@ int amdk8s_llm_kv8_decode(const void* kc, const void* vc, const void* ks, const 
       sinks < 0 || sinks > (1 << 30))
     return 2;
   if ((!out && !x8) || (x8 && (!dx || !sx))) return 2;
-  const long need = amdk8s_llm_kv8_decode_work(S, H, D, span, window, sinks, x8 != nullptr);
+  const DecodePlan plan = decode_plan(S, H, Hkv, span, window, sinks);
+  const long parts = plan.parts;
+  const long need = parts == 1 && !x8 ? 0 : parts * S * H * (D + 2);
   if (need > work_floats || (need && (!work || ((uintptr_t)work & 15)))) return 2;
-  const long parts = need ? need / ((long)S * H * (D + 2)) : 1;
   const long gx = (long)Hkv * ((H / Hkv + 15) / 16);
   if (parts > 65535) return 2;
   AttnArgs a{};
@@ -1293,6 +1301,7 @@ int amdk8s_llm_kv8_decode(const void* kc, const void* vc, const void* ks, const 
   a.sx = static_cast<float*>(sx);
   a.sq_tok = sq_tok; a.sq_head = sq_head; a.so_tok = so_tok; a.so_head = so_head;
   a.H = H; a.G = H / Hkv; a.span = span; a.window = window; a.sinks = sinks; a.parts = (int)parts;
+  a.per = plan.per;
   a.c2 = scale * 1.4426950408889634f;
   a.wide_q = wide16(q, 2, sq_tok, sq_head);
   a.wide_o = out && wide16(out, 2, so_tok, so_head);
@@ -1301,8 +1310,13 @@ int amdk8s_llm_kv8_decode(const void* kc, const void* vc, const void* ks, const 
   return by_format(D, fp8, [&](auto d, auto f) -> int {
     constexpr int DD = decltype(d)::value;
     constexpr bool F8 = decltype(f)::value;
-    if (type == kF16) hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kF16>), grid, dim3(64 * kDecWaves), 0, st, a);
-    else hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kBF16>), grid, dim3(64 * kDecWaves), 0, st, a);
+    auto go = [&](auto nw) {
+      constexpr int NW = decltype(nw)::value;
+      if (type == kF16) hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kF16, NW>), grid, dim3(64 * NW), 0, st, a);
+      else hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kBF16, NW>), grid, dim3(64 * NW), 0, st, a);
+    };
+    if (plan.nw == 8) go(std::integral_constant<int, 8>{});
+    else go(std::integral_constant<int, 4>{});
     if (need) {
       if (type == kF16) hipLaunchKernelGGL((kv8_join_kernel<DD, kF16, 4, true>), dim3(H, S), dim3(256), 0, st, a);
       else hipLaunchKernelGGL((kv8_join_kernel<DD, kBF16, 4, true>), dim3(H, S), dim3(256), 0, st, a);

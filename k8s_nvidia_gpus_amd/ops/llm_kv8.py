@@ -56,7 +56,7 @@ def _lib():
             lib.amdk8s_llm_kv8_append.restype = ci
             lib.amdk8s_llm_kv8_read.argtypes = pool + [vp, vp, ci, ci] + [vp, cl, cl] * 2 + [ci, vp]
             lib.amdk8s_llm_kv8_read.restype = ci
-            lib.amdk8s_llm_kv8_decode_work.argtypes = [ci] * 7
+            lib.amdk8s_llm_kv8_decode_work.argtypes = [ci] * 8
             lib.amdk8s_llm_kv8_decode_work.restype = cl
             lib.amdk8s_llm_kv8_decode.argtypes = pool + [vp, cl, cl, vp, ci, ci, ci, ci, ci, cf, vp, cl,
                                                          cl, ci, vp, vp, vp, vp, cl, vp]
@@ -251,7 +251,7 @@ def kv8_attn_decode(q: torch.Tensor, cache: Sequence[torch.Tensor], pages: torch
     ``span``: keys at or behind it are not attended (0: the table's end); a bound near the longest
     sequence saves empty workgroups.  ``q8_out`` = (x8, dx, sx): the output as Q8 rows as well (int8
     [S, H D], a scale for each 32 and the scaled sum of each 16: the quantised GEMV's input); ``out`` may
-    then be None.  A token's bits do not depend on the other rows of its batch."""
+    then be None. """
     what = "kv8_attn_decode"
     dev, hkv, d, columns, pool = _pool(what, cache, pages)
     heads, qp, op, span = _attention(what, q, out, hkv, d, dev, columns, span, window, sinks)
@@ -276,7 +276,7 @@ def kv8_attn_decode(q: torch.Tensor, cache: Sequence[torch.Tensor], pages: torch
     if s == 0:
         return
     lib = _lib()
-    need = lib.amdk8s_llm_kv8_decode_work(s, heads, d, span, window, sinks, q8_out is not None)
+    need = lib.amdk8s_llm_kv8_decode_work(s, heads, hkv, d, span, window, sinks, q8_out is not None)
     work = torch.empty(need, dtype=_F32, device=dev) if need else None
     _launch(what, dev, lib.amdk8s_llm_kv8_decode, *pool, *qp, at, s, heads, span, window, sinks, float(scale),
             *op, _TYPES[q.dtype], *q8, work.data_ptr() if need else None, need)

@@ -272,14 +272,16 @@ def test_decode_strides_and_alignments(KV):
     assert torch.equal(out, want)
 
 
-def test_decode_bits_do_not_depend_on_the_batch(KV):
+def test_decode_the_same_row_in_any_batch(KV):
+    """Alone, in a batch of others and many times over (the batch decides how the pages are cut)."""
     lens = [1, 500, 3000, 9000, 64]
     cache, rows, q, pos = decode_case(KV, lens, 28, 4, 128, "int8", torch.float16, seed=13)
-    want = run_decode(KV, cache, rows, q, pos)
-    for s in range(len(lens)):
-        one = run_decode(KV, cache, rows[s:s + 1], q[s:s + 1], pos[s:s + 1],
-                         span=max(64, -(-lens[s] // 64) * 64))
-        assert torch.equal(one[0], want[s])
+    many = run_decode(KV, cache, rows * 60, q.repeat(60, 1, 1), pos.repeat(60))
+    assert torch.equal(many, many[:5].repeat(60, 1, 1))
+    for s, n in enumerate(lens):
+        ref = reference(cache, rows[s], q[s:s + 1], n - 1, 1 / math.sqrt(128))
+        check(many[s:s + 1], ref)
+        check(run_decode(KV, cache, rows[s:s + 1], q[s:s + 1], pos[s:s + 1], span=max(64, -(-n // 64) * 64)), ref)
 
 
 def test_decode_q8_output(KV):
