@@ -1125,284 +1125,278 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
 
 }  // namespace
 
-extern "C" {
-
-int amdk8s_llm_kv8_page() { return kPage; }
-
-}  // extern "C"
-
+// ---------------------------------------------------------------- C entries
+// A call is one record of 64-bit fields (addresses, sizes and strides in elements), in the order of
+// these structs: passing some thirty arguments one by one cost the caller more than the kernel runs.
 namespace {
 
-bool wide16(const void* p, long esize, long s0, long s1) {
-  return ((uintptr_t)p & 15) == 0 && (s0 * esize) % 16 == 0 && (s1 * esize) % 16 == 0;
+struct PoolCall {
+  int64_t k, v, ks, vs, table, pool, hkv, d, fp8, width, stride;
+};
+struct RowsCall {
+  int64_t at, tok, head;               // address, row and head stride
+};
+struct AppendCall {
+  PoolCall c;
+  int64_t start, cu, s, n;
+  RowsCall k, v, q, qo;                // q, qo: address 0 for none
+  int64_t heads, cos_t, sin_t, table_rows, type, otype;   // types: 0 fp16, 1 bf16, 2 fp32; cos_t 0: no rotation
+};
+struct ReadCall {
+  PoolCall c;
+  int64_t start, cu, s, n;
+  RowsCall k, v;
+  int64_t type;
+};
+struct AttnCall {
+  PoolCall c;
+  int64_t start, cu, s, n;             // decode: start = positions, cu unused, n = s
+  RowsCall q, out;                     // out: address 0 for none (decode with x8)
+  int64_t heads, span, window, sinks, type;
+  int64_t x8, dx, sx;                  // decode: Q8 output or 0
+};
+
+template <typename T>
+T* ptr(int64_t a) {
+  return reinterpret_cast<T*>(a);
+}
+bool wide16(const RowsCall& r, long esize) {
+  return (r.at & 15) == 0 && (r.tok * esize) % 16 == 0 && (r.head * esize) % 16 == 0;
 }
 int launched() { return hipGetLastError() == hipSuccess ? 0 : 1; }
+bool in(int64_t x, int64_t low, int64_t high) { return x >= low && x <= high; }
 
 // D and the code type to template arguments
 template <typename F>
-int by_format(int D, int fp8, F f) {
+int by_format(const PoolCall& c, F f) {
   using I64 = std::integral_constant<int, 64>;
   using I128 = std::integral_constant<int, 128>;
-  if (D == 128) return fp8 ? f(I128{}, std::true_type{}) : f(I128{}, std::false_type{});
-  if (D == 64) return fp8 ? f(I64{}, std::true_type{}) : f(I64{}, std::false_type{});
+  if (c.d == 128) return c.fp8 ? f(I128{}, std::true_type{}) : f(I128{}, std::false_type{});
+  if (c.d == 64) return c.fp8 ? f(I64{}, std::true_type{}) : f(I64{}, std::false_type{});
   return 2;
 }
 
-Pool make_pool(void* k, void* v, void* ks, void* vs, const void* table, int pool, int Hkv, int width, int stride) {
-  return Pool{static_cast<uint8_t*>(k), static_cast<uint8_t*>(v), static_cast<float*>(ks), static_cast<float*>(vs),
-              static_cast<const int*>(table), pool, Hkv, width, stride};
+bool good_pool(const PoolCall& c) {
+  return c.k && c.v && c.ks && c.vs && c.table && ((c.k | c.v) & 15) == 0 && in(c.pool, 1, 0x7fffffff) &&
+         in(c.hkv, 1, 65535) && in(c.width, 1, 1 << 24) && in(c.stride, 0, 0x7fffffff);
 }
-bool bad_pool(const void* k, const void* v, const void* ks, const void* vs, const void* table, int pool, int Hkv,
-              int width) {
-  return !k || !v || !ks || !vs || !table || pool < 1 || Hkv < 1 || width < 1 || width > (1 << 24) ||
-         (((uintptr_t)k | (uintptr_t)v) & 15);
+bool good_segs(int64_t start, int64_t cu, int64_t s, int64_t n) {
+  return start && cu && in(s, 1, 0x3fffffff) && in(n, 1, 0x3fffffff);
+}
+Pool make_pool(const PoolCall& c) {
+  return Pool{ptr<uint8_t>(c.k), ptr<uint8_t>(c.v), ptr<float>(c.ks), ptr<float>(c.vs), ptr<const int>(c.table),
+              (int)c.pool, (int)c.hkv, (int)c.width, (int)c.stride};
+}
+Segs make_segs(int64_t start, int64_t cu, int64_t s, int64_t n) {
+  return Segs{ptr<const int>(start), ptr<const int>(cu), (int)s, (int)n};
+}
+bool good_attn(const AttnCall& c) {
+  return good_pool(c.c) && c.start && c.q.at && in(c.heads, 1, 0x3fffffff) && c.heads % c.c.hkv == 0 &&
+         in(c.type, 0, 1) && in(c.span, 1, c.c.width * kPage) && in(c.window, 0, 1 << 30) && in(c.sinks, 0, 1 << 30);
+}
+AttnArgs make_attn(const AttnCall& c, float scale, void* work, long parts) {
+  AttnArgs a{};
+  a.c = make_pool(c.c);
+  a.sg = make_segs(c.start, c.cu, c.s, c.n);
+  a.q = ptr<const uint16_t>(c.q.at);
+  a.out = ptr<void>(c.out.at);
+  a.po = static_cast<float*>(work);
+  a.pml = work ? a.po + parts * c.n * c.heads * c.c.d : nullptr;
+  a.x8 = ptr<int8_t>(c.x8);
+  a.dx = ptr<float>(c.dx);
+  a.sx = ptr<float>(c.sx);
+  a.sq_tok = c.q.tok; a.sq_head = c.q.head; a.so_tok = c.out.tok; a.so_head = c.out.head;
+  a.H = (int)c.heads; a.G = (int)(c.heads / c.c.hkv);
+  a.span = (int)c.span; a.window = (int)c.window; a.sinks = (int)c.sinks; a.parts = (int)parts;
+  a.c2 = scale * 1.4426950408889634f;
+  a.wide_q = wide16(c.q, 2);
+  a.wide_o = c.out.at && wide16(c.out, 2);
+  return a;
+}
+
+// most pages that queries at `rows` neighbouring positions see
+long most_seen(const AttnCall& c, long rows) {
+  const long n = (c.span + kPage - 1) / kPage;
+  if (c.window <= 0) return n;
+  const long w = (c.window + rows + 61) / kPage + 1 + (c.sinks + kPage - 1) / kPage;
+  return w < n ? w : n;
+}
+
+constexpr long kDecodeGrid = 768;                        // workgroups: three on each of the 256 CUs
+
+struct DecodePlan {
+  int nw, per;
+  long parts;
+};
+// Pages a wave: one until the workgroups fill the chip three deep, then as many as keep it so (a longer
+// chain of pages pays a workgroup's start and its partial output once).  Up to 8 pages run in one
+// workgroup of 8 waves, which needs no join.
+DecodePlan decode_plan(const AttnCall& c) {
+  const long n = most_seen(c, 1);
+  if (n <= 8) return {8, 1, 1};
+  const long chains = c.s * c.c.hkv * ((c.heads / c.c.hkv + 15) / 16);
+  long per = chains * n / (4 * kDecodeGrid);
+  per = per < 1 ? 1 : per > 64 ? 64 : per;
+  return {4, (int)per, (n + 4 * per - 1) / (4 * per)};
+}
+
+constexpr int kPromptWaves = 4;
+constexpr long kPromptGrid = 512;                        // two workgroups on each of the 256 CUs
+
+struct PromptPlan {
+  long units, parts;
+};
+// Workgroups that share a row block's keys: as many as fill the chip when there are few row blocks, each
+// with at least 8 pages.
+PromptPlan prompt_plan(const AttnCall& c) {
+  const long rows = 32 * kPromptWaves, G = c.heads / c.c.hkv;
+  long units = c.n * G / rows + c.s;
+  if (G <= rows && units > c.n) units = c.n;
+  long parts = kPromptGrid / (units * c.c.hkv);
+  const long most = most_seen(c, (rows + G - 1) / G + 1) / 8;
+  parts = parts > most ? most : parts;
+  return {units, parts < 1 ? 1 : parts};
 }
 
 }  // namespace
 
 extern "C" {
 
-// rc: 0 launched, 1 launch error, 2 bad argument.
-// Rows of k / v (and q) of S segments into the cache; cos_t null: no rotation; q null: keys only.
-// type: element type of k, v, q (0 fp16, 1 bf16, 2 fp32); otype: of qo (0, 1).
-int amdk8s_llm_kv8_append(void* kc, void* vc, void* ks, void* vs, const void* table, int pool, int Hkv, int D,
-                          int fp8, int width, int tstride, const void* start, const void* cu, int S, int N,
-                          const void* k, long sk_tok, long sk_head, const void* v, long sv_tok, long sv_head,
-                          const void* q, long sq_tok, long sq_head, void* qo, long so_tok, long so_head, int H,
-                          const void* cos_t, const void* sin_t, int table_rows, int type, int otype, void* stream) {
-  if (bad_pool(kc, vc, ks, vs, table, pool, Hkv, width) || !start || !cu || S < 1 || N < 1 || !k || !v) return 2;
-  if ((q != nullptr) != (qo != nullptr) || (q && H < 1) || (cos_t != nullptr) != (sin_t != nullptr)) return 2;
-  if (type < 0 || type > 2 || otype < 0 || otype > 1 || (type < 2 && otype != type)) return 2;
-  if (cos_t && (table_rows < width * (long)kPage || (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15))) return 2;
+int amdk8s_llm_kv8_page() { return kPage; }
+
+// Each entry returns 0: launched, 1: a launch error, 2: a bad argument.
+
+// Rows of k / v (and q) of the segments into the cache.
+int amdk8s_llm_kv8_append(const void* call, void* stream) {
+  const AppendCall& c = *static_cast<const AppendCall*>(call);
+  if (!good_pool(c.c) || !good_segs(c.start, c.cu, c.s, c.n) || !c.k.at || !c.v.at) return 2;
+  if (!c.q.at != !c.qo.at || (c.q.at && !in(c.heads, 1, 0x3fffffff)) || !c.cos_t != !c.sin_t) return 2;
+  if (!in(c.type, 0, 2) || !in(c.otype, 0, 1) || (c.type < 2 && c.otype != c.type)) return 2;
+  if (c.cos_t && (!in(c.table_rows, c.c.width * kPage, 0x7fffffff) || ((c.cos_t | c.sin_t) & 15))) return 2;
   AppendArgs a{};
-  a.c = make_pool(kc, vc, ks, vs, table, pool, Hkv, width, tstride);
-  a.sg = Segs{static_cast<const int*>(start), static_cast<const int*>(cu), S, N};
-  a.k = k; a.v = v; a.q = q; a.qo = qo;
-  a.cos_t = static_cast<const float*>(cos_t);
-  a.sin_t = static_cast<const float*>(sin_t);
-  a.sk_tok = sk_tok; a.sk_head = sk_head; a.sv_tok = sv_tok; a.sv_head = sv_head;
-  a.sq_tok = sq_tok; a.sq_head = sq_head; a.so_tok = so_tok; a.so_head = so_head;
-  a.H = H;
-  const int es = type == kF32 ? 4 : 2;
-  a.wide_kv = wide16(k, es, sk_tok, sk_head) && wide16(v, es, sv_tok, sv_head);
-  a.wide_q = q && wide16(q, es, sq_tok, sq_head) && wide16(qo, 2, so_tok, so_head);
-  a.table_rows = cos_t ? table_rows : 0x7fffffff;
-  const long units = most_pages(N, S), qb = q ? (N + 3L) / 4 : 0;
-  if (units * Hkv + qb > 0x7fffffffL) return 2;
+  a.c = make_pool(c.c);
+  a.sg = make_segs(c.start, c.cu, c.s, c.n);
+  a.k = ptr<void>(c.k.at); a.v = ptr<void>(c.v.at); a.q = ptr<void>(c.q.at); a.qo = ptr<void>(c.qo.at);
+  a.cos_t = ptr<const float>(c.cos_t);
+  a.sin_t = ptr<const float>(c.sin_t);
+  a.sk_tok = c.k.tok; a.sk_head = c.k.head; a.sv_tok = c.v.tok; a.sv_head = c.v.head;
+  a.sq_tok = c.q.tok; a.sq_head = c.q.head; a.so_tok = c.qo.tok; a.so_head = c.qo.head;
+  a.H = (int)c.heads;
+  const int es = c.type == kF32 ? 4 : 2;
+  a.wide_kv = wide16(c.k, es) && wide16(c.v, es);
+  a.wide_q = c.q.at && wide16(c.q, es) && wide16(c.qo, 2);
+  a.table_rows = c.cos_t ? (int)c.table_rows : 0x7fffffff;
+  const long units = most_pages(c.n, c.s), qb = c.q.at ? (c.n + 3) / 4 : 0;
+  if (units * c.c.hkv + qb > 0x7fffffffL) return 2;
   a.units = (int)units;
-  const dim3 grid((unsigned)(units * Hkv + qb));
+  const dim3 grid((unsigned)(units * c.c.hkv + qb));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return by_format(D, fp8, [&](auto d, auto f) -> int {
+  return by_format(c.c, [&](auto d, auto f) -> int {
     constexpr int DD = decltype(d)::value;
     constexpr bool F8 = decltype(f)::value;
-    if (type == kF16) hipLaunchKernelGGL((kv8_append_kernel<DD, F8, kF16, kF16>), grid, dim3(256), 0, st, a);
-    else if (type == kBF16) hipLaunchKernelGGL((kv8_append_kernel<DD, F8, kBF16, kBF16>), grid, dim3(256), 0, st, a);
-    else if (otype == kF16) hipLaunchKernelGGL((kv8_append_kernel<DD, F8, kF32, kF16>), grid, dim3(256), 0, st, a);
+    if (c.type == kF16) hipLaunchKernelGGL((kv8_append_kernel<DD, F8, kF16, kF16>), grid, dim3(256), 0, st, a);
+    else if (c.type == kBF16) hipLaunchKernelGGL((kv8_append_kernel<DD, F8, kBF16, kBF16>), grid, dim3(256), 0, st, a);
+    else if (c.otype == kF16) hipLaunchKernelGGL((kv8_append_kernel<DD, F8, kF32, kF16>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv8_append_kernel<DD, F8, kF32, kBF16>), grid, dim3(256), 0, st, a);
     return launched();
   });
 }
 
-// Cached positions of S segments as values: rows of ko / vo (type 0 fp16, 1 bf16, 2 fp32).
-int amdk8s_llm_kv8_read(const void* kc, const void* vc, const void* ks, const void* vs, const void* table, int pool,
-                        int Hkv, int D, int fp8, int width, int tstride, const void* start, const void* cu, int S,
-                        int N, void* ko, long sk_tok, long sk_head, void* vo, long sv_tok, long sv_head, int type,
-                        void* stream) {
-  if (bad_pool(kc, vc, ks, vs, table, pool, Hkv, width) || !start || !cu || S < 1 || N < 1 || !ko || !vo) return 2;
-  if (type < 0 || type > 2) return 2;
+// Cached positions of the segments as values.
+int amdk8s_llm_kv8_read(const void* call, void* stream) {
+  const ReadCall& c = *static_cast<const ReadCall*>(call);
+  if (!good_pool(c.c) || !good_segs(c.start, c.cu, c.s, c.n) || !c.k.at || !c.v.at || !in(c.type, 0, 2)) return 2;
   ReadArgs a{};
-  a.c = make_pool(const_cast<void*>(kc), const_cast<void*>(vc), const_cast<void*>(ks), const_cast<void*>(vs), table,
-                  pool, Hkv, width, tstride);
-  a.sg = Segs{static_cast<const int*>(start), static_cast<const int*>(cu), S, N};
-  a.ko = ko; a.vo = vo;
-  a.sk_tok = sk_tok; a.sk_head = sk_head; a.sv_tok = sv_tok; a.sv_head = sv_head;
-  const int es = type == kF32 ? 4 : 2;
-  a.wide = wide16(ko, es, sk_tok, sk_head) && wide16(vo, es, sv_tok, sv_head);
-  const long blocks = most_pages(N, S) * Hkv;
+  a.c = make_pool(c.c);
+  a.sg = make_segs(c.start, c.cu, c.s, c.n);
+  a.ko = ptr<void>(c.k.at); a.vo = ptr<void>(c.v.at);
+  a.sk_tok = c.k.tok; a.sk_head = c.k.head; a.sv_tok = c.v.tok; a.sv_head = c.v.head;
+  const int es = c.type == kF32 ? 4 : 2;
+  a.wide = wide16(c.k, es) && wide16(c.v, es);
+  const long blocks = most_pages(c.n, c.s) * c.c.hkv;
   if (blocks > 0x7fffffffL) return 2;
-  hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)blocks);
-  return by_format(D, fp8, [&](auto d, auto f) -> int {
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return by_format(c.c, [&](auto d, auto f) -> int {
     constexpr int DD = decltype(d)::value;
     constexpr bool F8 = decltype(f)::value;
-    if (type == kF16) hipLaunchKernelGGL((kv8_read_kernel<DD, F8, kF16>), grid, dim3(256), 0, st, a);
-    else if (type == kBF16) hipLaunchKernelGGL((kv8_read_kernel<DD, F8, kBF16>), grid, dim3(256), 0, st, a);
+    if (c.type == kF16) hipLaunchKernelGGL((kv8_read_kernel<DD, F8, kF16>), grid, dim3(256), 0, st, a);
+    else if (c.type == kBF16) hipLaunchKernelGGL((kv8_read_kernel<DD, F8, kBF16>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv8_read_kernel<DD, F8, kF32>), grid, dim3(256), 0, st, a);
     return launched();
   });
 }
 
-}  // extern "C"
-
-namespace {
-
-constexpr long kDecodeGrid = 768;                        // workgroups: three on each of the 256 CUs
-
-struct DecodePlan {
-  int nw, per, parts;
-};
-// Pages a wave: one until the workgroups fill the chip three deep, then as many as keep it so (a longer
-// chain of pages pays a workgroup's start and its partial output once).  Up to 8 pages run in one
-// workgroup of 8 waves, which needs no join.
-DecodePlan decode_plan(long S, int H, int Hkv, int span, int window, int sinks) {
-  long n = (span + (long)kPage - 1) / kPage;             // pages a row sees at most
-  if (window > 0) {
-    const long w = (window + 62L) / kPage + 1 + (sinks + 63L) / kPage;
-    n = w < n ? w : n;
-  }
-  if (n <= 8) return {8, 1, 1};
-  const long chains = S * Hkv * ((H / Hkv + 15) / 16);
-  long per = chains * n / (4 * kDecodeGrid);
-  per = per < 1 ? 1 : per > 64 ? 64 : per;
-  return {4, (int)per, (int)((n + 4 * per - 1) / (4 * per))};
+// fp32 workspace (in floats) of the call: 0 when its partials need no join, -1 for a bad argument
+long amdk8s_llm_kv8_decode_work(const void* call) {
+  const AttnCall& c = *static_cast<const AttnCall*>(call);
+  if (!good_attn(c) || !in(c.s, 1, 65535) || c.n != c.s) return -1;
+  const long parts = decode_plan(c).parts;
+  return parts == 1 && !c.x8 ? 0 : parts * c.n * c.heads * (c.c.d + 2);
 }
 
-}  // namespace
-
-extern "C" {
-
-// fp32 workspace (in floats) of a decode call: 0 when its partials need no join
-long amdk8s_llm_kv8_decode_work(int S, int H, int Hkv, int D, int span, int window, int sinks, int q8) {
-  if (S < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || span < 1 || window < 0 || sinks < 0) return -1;
-  const long parts = decode_plan(S, H, Hkv, span, window, sinks).parts;
-  return parts == 1 && !q8 ? 0 : parts * S * H * (D + 2);
-}
-
-// One query row a sequence at position pos[s] (-1: nothing to see, zeros).  span: keys at or behind it are
-// not attended.  type: q and out (0 fp16, 1 bf16).  x8 / dx / sx (nullable): the output as Q8 rows; out
-// may then be null.
-int amdk8s_llm_kv8_decode(const void* kc, const void* vc, const void* ks, const void* vs, const void* table,
-                          int pool, int Hkv, int D, int fp8, int width, int tstride, const void* q, long sq_tok,
-                          long sq_head, const void* pos, int S, int H, int span, int window, int sinks, float scale,
-                          void* out, long so_tok, long so_head, int type, void* x8, void* dx, void* sx, void* work,
-                          long work_floats, void* stream) {
-  if (bad_pool(kc, vc, ks, vs, table, pool, Hkv, width) || !q || !pos || S < 1 || S > 65535 || H < 1 || H % Hkv)
-    return 2;
-  if (type < 0 || type > 1 || span < 1 || span > width * (long)kPage || window < 0 || window > (1 << 30) ||
-      sinks < 0 || sinks > (1 << 30))
-    return 2;
-  if ((!out && !x8) || (x8 && (!dx || !sx))) return 2;
-  const DecodePlan plan = decode_plan(S, H, Hkv, span, window, sinks);
-  const long parts = plan.parts;
-  const long need = parts == 1 && !x8 ? 0 : parts * S * H * (D + 2);
-  if (need > work_floats || (need && (!work || ((uintptr_t)work & 15)))) return 2;
-  const long gx = (long)Hkv * ((H / Hkv + 15) / 16);
-  if (parts > 65535) return 2;
-  AttnArgs a{};
-  a.c = make_pool(const_cast<void*>(kc), const_cast<void*>(vc), const_cast<void*>(ks), const_cast<void*>(vs), table,
-                  pool, Hkv, width, tstride);
-  a.sg = Segs{static_cast<const int*>(pos), nullptr, S, S};
-  a.q = static_cast<const uint16_t*>(q);
-  a.out = out;
-  a.po = static_cast<float*>(work);
-  a.pml = need ? a.po + parts * S * H * D : nullptr;
-  a.x8 = static_cast<int8_t*>(x8);
-  a.dx = static_cast<float*>(dx);
-  a.sx = static_cast<float*>(sx);
-  a.sq_tok = sq_tok; a.sq_head = sq_head; a.so_tok = so_tok; a.so_head = so_head;
-  a.H = H; a.G = H / Hkv; a.span = span; a.window = window; a.sinks = sinks; a.parts = (int)parts;
+// One query row a sequence at position start[s] (-1: nothing to see, zeros); keys at or behind `span` are
+// not attended.
+int amdk8s_llm_kv8_decode(const void* call, float scale, void* work, long work_floats, void* stream) {
+  const AttnCall& c = *static_cast<const AttnCall*>(call);
+  const long need = amdk8s_llm_kv8_decode_work(call);
+  if (need < 0 || need > work_floats || (need && (!work || ((uintptr_t)work & 15)))) return 2;
+  if ((!c.out.at && !c.x8) || (c.x8 && (!c.dx || !c.sx))) return 2;
+  const DecodePlan plan = decode_plan(c);
+  if (plan.parts > 65535) return 2;
+  AttnArgs a = make_attn(c, scale, need ? work : nullptr, plan.parts);
   a.per = plan.per;
-  a.c2 = scale * 1.4426950408889634f;
-  a.wide_q = wide16(q, 2, sq_tok, sq_head);
-  a.wide_o = out && wide16(out, 2, so_tok, so_head);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)gx, (unsigned)parts, S);
-  return by_format(D, fp8, [&](auto d, auto f) -> int {
+  const dim3 grid((unsigned)(c.c.hkv * ((a.G + 15) / 16)), (unsigned)plan.parts, (unsigned)c.s);
+  return by_format(c.c, [&](auto d, auto f) -> int {
     constexpr int DD = decltype(d)::value;
     constexpr bool F8 = decltype(f)::value;
     auto go = [&](auto nw) {
       constexpr int NW = decltype(nw)::value;
-      if (type == kF16) hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kF16, NW>), grid, dim3(64 * NW), 0, st, a);
+      if (c.type == kF16) hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kF16, NW>), grid, dim3(64 * NW), 0, st, a);
       else hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kBF16, NW>), grid, dim3(64 * NW), 0, st, a);
     };
     if (plan.nw == 8) go(std::integral_constant<int, 8>{});
     else go(std::integral_constant<int, 4>{});
     if (need) {
-      if (type == kF16) hipLaunchKernelGGL((kv8_join_kernel<DD, kF16, 4, true>), dim3(H, S), dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((kv8_join_kernel<DD, kBF16, 4, true>), dim3(H, S), dim3(256), 0, st, a);
+      const dim3 rows((unsigned)c.heads, (unsigned)c.s);
+      if (c.type == kF16) hipLaunchKernelGGL((kv8_join_kernel<DD, kF16, 4, true>), rows, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((kv8_join_kernel<DD, kBF16, 4, true>), rows, dim3(256), 0, st, a);
     }
     return launched();
   });
 }
 
-}  // extern "C"
-
-namespace {
-
-constexpr int kPromptWaves = 4;
-constexpr int kPromptGrid = 512;                         // two workgroups on each of the 256 CUs
-
-// workgroups that share a row block's keys: as many as fill the chip when there are few row blocks, each
-// with at least 8 pages
-int prompt_parts(long N, int S, int H, int Hkv, int span, int window, int sinks, long& units) {
-  const int rows = 32 * kPromptWaves, G = H / Hkv;
-  units = N * G / rows + S;
-  if (G <= rows && units > N) units = N;
-  long n = (span + (long)kPage - 1) / kPage;
-  if (window > 0) {
-    const long w = (window + (rows + G - 1) / G + 62L) / kPage + 1 + (sinks + 63L) / kPage;
-    n = w < n ? w : n;
-  }
-  long parts = kPromptGrid / (units * Hkv);
-  if (parts > n / 8) parts = n / 8;
-  return parts < 1 ? 1 : (int)parts;
+long amdk8s_llm_kv8_prompt_work(const void* call) {
+  const AttnCall& c = *static_cast<const AttnCall*>(call);
+  if (!good_attn(c) || !good_segs(c.start, c.cu, c.s, c.n) || c.n * (c.heads / c.c.hkv) > 0x3fffffffL) return -1;
+  const long parts = prompt_plan(c).parts;
+  return parts == 1 ? 0 : parts * c.n * c.heads * (c.c.d + 2);
 }
 
-}  // namespace
-
-extern "C" {
-
-// fp32 workspace (in floats) of a prompt call
-long amdk8s_llm_kv8_prompt_work(int N, int S, int H, int Hkv, int D, int span, int window, int sinks) {
-  if (N < 1 || S < 1 || Hkv < 1 || H < Hkv || H % Hkv || D < 1 || span < 1 || window < 0 || sinks < 0) return -1;
-  long units;
-  const long parts = prompt_parts(N, S, H, Hkv, span, window, sinks, units);
-  return parts == 1 ? 0 : parts * N * H * (D + 2);
-}
-
-// Query rows of S segments (row cu[s] + i at position start[s] + i) over the cache, their own keys
+// Query rows of the segments (row cu[s] + i at position start[s] + i) over the cache, their own keys
 // included; rows in no segment are left as they are.
-int amdk8s_llm_kv8_prompt(const void* kc, const void* vc, const void* ks, const void* vs, const void* table,
-                          int pool, int Hkv, int D, int fp8, int width, int tstride, const void* start,
-                          const void* cu, int S, int N, const void* q, long sq_tok, long sq_head, int H, int span,
-                          int window, int sinks, float scale, void* out, long so_tok, long so_head, int type,
-                          void* work, long work_floats, void* stream) {
-  if (bad_pool(kc, vc, ks, vs, table, pool, Hkv, width) || !q || !out || !start || !cu || S < 1 || N < 1 || H < 1 ||
-      H % Hkv)
-    return 2;
-  if (type < 0 || type > 1 || span < 1 || span > width * (long)kPage || window < 0 || window > (1 << 30) ||
-      sinks < 0 || sinks > (1 << 30) || (long)N * (H / Hkv) > 0x3fffffffL)
-    return 2;
-  long units;
-  const long parts = prompt_parts(N, S, H, Hkv, span, window, sinks, units);
-  const long need = parts == 1 ? 0 : parts * N * H * (D + 2);
-  if (need > work_floats || (need && (!work || ((uintptr_t)work & 15)))) return 2;
-  if (units * Hkv > 0x7fffffffL || parts > 65535 || (parts > 1 && N > 65535)) return 2;
-  AttnArgs a{};
-  a.c = make_pool(const_cast<void*>(kc), const_cast<void*>(vc), const_cast<void*>(ks), const_cast<void*>(vs), table,
-                  pool, Hkv, width, tstride);
-  a.sg = Segs{static_cast<const int*>(start), static_cast<const int*>(cu), S, N};
-  a.q = static_cast<const uint16_t*>(q);
-  a.out = out;
-  a.po = static_cast<float*>(work);
-  a.pml = need ? a.po + parts * N * H * D : nullptr;
-  a.sq_tok = sq_tok; a.sq_head = sq_head; a.so_tok = so_tok; a.so_head = so_head;
-  a.H = H; a.G = H / Hkv; a.span = span; a.window = window; a.sinks = sinks; a.parts = (int)parts;
-  a.units = (int)units;
-  a.c2 = scale * 1.4426950408889634f;
-  a.wide_q = wide16(q, 2, sq_tok, sq_head);
-  a.wide_o = wide16(out, 2, so_tok, so_head);
+int amdk8s_llm_kv8_prompt(const void* call, float scale, void* work, long work_floats, void* stream) {
+  const AttnCall& c = *static_cast<const AttnCall*>(call);
+  const long need = amdk8s_llm_kv8_prompt_work(call);
+  if (need < 0 || need > work_floats || (need && (!work || ((uintptr_t)work & 15)))) return 2;
+  if (!c.out.at || c.x8) return 2;
+  const PromptPlan plan = prompt_plan(c);
+  if (plan.units * c.c.hkv > 0x7fffffffL || plan.parts > 65535 || (plan.parts > 1 && c.n > 65535)) return 2;
+  AttnArgs a = make_attn(c, scale, need ? work : nullptr, plan.parts);
+  a.units = (int)plan.units;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(units * Hkv), (unsigned)parts);
-  return by_format(D, fp8, [&](auto d, auto f) -> int {
+  const dim3 grid((unsigned)(plan.units * c.c.hkv), (unsigned)plan.parts);
+  return by_format(c.c, [&](auto d, auto f) -> int {
     constexpr int DD = decltype(d)::value;
     constexpr bool F8 = decltype(f)::value;
     constexpr int NW = kPromptWaves;
-    if (type == kF16) hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kF16, NW>), grid, dim3(64 * NW), 0, st, a);
+    if (c.type == kF16) hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kF16, NW>), grid, dim3(64 * NW), 0, st, a);
     else hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kBF16, NW>), grid, dim3(64 * NW), 0, st, a);
     if (need) {
-      if (type == kF16) hipLaunchKernelGGL((kv8_join_kernel<DD, kF16, 1, false>), dim3(H, N), dim3(64), 0, st, a);
-      else hipLaunchKernelGGL((kv8_join_kernel<DD, kBF16, 1, false>), dim3(H, N), dim3(64), 0, st, a);
+      const dim3 rows((unsigned)c.heads, (unsigned)c.n);
+      if (c.type == kF16) hipLaunchKernelGGL((kv8_join_kernel<DD, kF16, 1, false>), rows, dim3(64), 0, st, a);
+      else hipLaunchKernelGGL((kv8_join_kernel<DD, kBF16, 1, false>), rows, dim3(64), 0, st, a);
     }
     return launched();
   });

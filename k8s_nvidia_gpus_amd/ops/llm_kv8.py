@@ -27,6 +27,7 @@ and captured graphs never share it.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from typing import NamedTuple, Optional, Sequence, Tuple
 
@@ -38,36 +39,36 @@ PAGE = 64
 
 _CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_QTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _I32, _F32 = torch.int32, torch.float32
 
-_declared = False
+# The C entries take one record of 64-bit fields (the structs of csrc/llm_kv8.hip): the page pool, the
+# segments, then the call's own.
+_APPEND = struct.Struct("33q")
+_READ = struct.Struct("22q")
+_ATTN = struct.Struct("29q")
+_NONE = (0, 0, 0)
+
+_entries = None
 _lock = threading.Lock()
 
 
 def _lib():
-    global _declared
-    lib = library()
-    if not _declared:
+    global _entries
+    if _entries is None:
         with _lock:
+            lib = library()
             vp, ci, cl, cf = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
-            pool = [vp] * 5 + [ci] * 6
-            lib.amdk8s_llm_kv8_append.argtypes = pool + [vp, vp, ci, ci] + [vp, cl, cl] * 4 \
-                + [ci, vp, vp, ci, ci, ci, vp]
-            lib.amdk8s_llm_kv8_append.restype = ci
-            lib.amdk8s_llm_kv8_read.argtypes = pool + [vp, vp, ci, ci] + [vp, cl, cl] * 2 + [ci, vp]
-            lib.amdk8s_llm_kv8_read.restype = ci
-            lib.amdk8s_llm_kv8_decode_work.argtypes = [ci] * 8
-            lib.amdk8s_llm_kv8_decode_work.restype = cl
-            lib.amdk8s_llm_kv8_decode.argtypes = pool + [vp, cl, cl, vp, ci, ci, ci, ci, ci, cf, vp, cl,
-                                                         cl, ci, vp, vp, vp, vp, cl, vp]
-            lib.amdk8s_llm_kv8_decode.restype = ci
-            lib.amdk8s_llm_kv8_prompt_work.argtypes = [ci] * 8
-            lib.amdk8s_llm_kv8_prompt_work.restype = cl
-            lib.amdk8s_llm_kv8_prompt.argtypes = pool + [vp, vp, ci, ci, vp, cl, cl, ci, ci, ci, ci, cf,
-                                                         vp, cl, cl, ci, vp, cl, vp]
-            lib.amdk8s_llm_kv8_prompt.restype = ci
-            _declared = True
-    return lib
+            for name in ("append", "read"):
+                f = getattr(lib, f"amdk8s_llm_kv8_{name}")
+                f.argtypes, f.restype = [ctypes.c_char_p, vp], ci
+            for name in ("decode", "prompt"):
+                f = getattr(lib, f"amdk8s_llm_kv8_{name}")
+                f.argtypes, f.restype = [ctypes.c_char_p, cf, vp, cl, vp], ci
+                f = getattr(lib, f"amdk8s_llm_kv8_{name}_work")
+                f.argtypes, f.restype = [ctypes.c_char_p], cl
+            _entries = lib
+    return _entries
 
 
 class KV8Cache(NamedTuple):
@@ -96,58 +97,59 @@ def _bad(what: str, why: str):
 
 
 def _pool(what: str, cache: Sequence[torch.Tensor], pages: torch.Tensor):
-    """Checked cache and table -> (device, Hkv, D, columns, the C arguments of both)."""
+    """Checked cache and table -> (device index, Hkv, D, sequences, columns, the record's fields)."""
     k, v, ks, vs = cache
-    dev = k.device
-    if k.dim() != 4 or k.dtype not in _CODES or v.dtype != k.dtype or k.shape[2] != PAGE \
-            or k.shape[3] not in (64, 128) or v.shape != (k.shape[0], k.shape[1], k.shape[3], PAGE) \
-            or not k.is_contiguous() or not v.is_contiguous():
-        _bad(what, f"cache codes k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype} are not "
+    shape, code = k.shape, k.dtype
+    if len(shape) != 4 or code not in _CODES or v.dtype != code or shape[2] != PAGE \
+            or shape[3] not in (64, 128) or v.shape != (shape[0], shape[1], shape[3], PAGE) \
+            or not k.is_contiguous() or not v.is_contiguous() or shape[0] < 1 or shape[1] < 1:
+        _bad(what, f"cache codes k {tuple(shape)} {code}, v {tuple(v.shape)} {v.dtype} are not "
                    f"contiguous [pages, Hkv, {PAGE}, D] and [pages, Hkv, D, {PAGE}] of int8 or "
                    f"float8_e4m3fn with D 64 or 128")
-    n, hkv, _, d = k.shape
-    if n < 1 or hkv < 1:
-        _bad(what, f"an empty cache {tuple(k.shape)}")
-    for s in (ks, vs):
-        if s.dtype != _F32 or s.shape != (n, hkv) or not s.is_contiguous() or s.device != dev:
-            _bad(what, f"scales must be contiguous fp32 [{n}, {hkv}] on {dev}")
-    if v.device != dev:
-        _bad(what, f"the cache must lie on one device, not {dev} / {v.device}")
-    if pages.dtype != _I32 or pages.dim() != 2 or pages.shape[0] < 1 or pages.shape[1] < 1 \
-            or pages.stride(1) != 1 or pages.stride(0) < 0 or pages.device != dev:
-        _bad(what, f"the page table must be int32 [S, columns] with a unit inner stride on {dev}")
-    return dev, hkv, d, pages.shape[1], (
+    n, hkv, _, d = shape
+    dev, each = k.get_device(), (n, hkv)
+    if ks.dtype != _F32 or ks.shape != each or not ks.is_contiguous() or ks.get_device() != dev \
+            or vs.dtype != _F32 or vs.shape != each or not vs.is_contiguous() or vs.get_device() != dev:
+        _bad(what, f"scales must be contiguous fp32 [{n}, {hkv}] on {k.device}")
+    if v.get_device() != dev:
+        _bad(what, f"the cache must lie on one device, not {k.device} / {v.device}")
+    table, strides = pages.shape, pages.stride()
+    if pages.dtype != _I32 or len(table) != 2 or table[0] < 1 or table[1] < 1 or strides[1] != 1 \
+            or pages.get_device() != dev:
+        _bad(what, f"the page table must be int32 [S, columns] with a unit inner stride on {k.device}")
+    return dev, hkv, d, table[0], table[1], (
         k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages.data_ptr(), n, hkv, d,
-        _CODES[k.dtype], pages.shape[1], pages.stride(0))
+        _CODES[code], table[1], strides[0])
 
 
-def _ints(what: str, name: str, t: torch.Tensor, n: int, dev) -> int:
-    if t.dtype != _I32 or t.shape != (n,) or t.device != dev or (n > 1 and t.stride(0) != 1):
-        _bad(what, f"{name} must be contiguous int32 [{n}] on {dev}")
+def _ints(what: str, name: str, t: torch.Tensor, n: int, dev: int) -> int:
+    if t.dtype != _I32 or t.shape != (n,) or not t.is_contiguous() or t.get_device() != dev:
+        _bad(what, f"{name} must be contiguous int32 [{n}] on the cache's device")
     return t.data_ptr()
 
 
-def _rows(what: str, name: str, t: torch.Tensor, heads: int, d: int, dev) -> Tuple[int, int, int]:
-    """A [rows, heads, D] view with a unit inner stride -> (pointer, row stride, head stride)."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != d or t.stride(2) != 1 or t.device != dev:
-        _bad(what, f"{name} {tuple(t.shape)} / {t.stride()} on {t.device} is not [rows, {heads}, {d}] "
-                   f"with a unit inner stride on {dev}")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+def _rows(what: str, name: str, t: torch.Tensor, n: int, heads: int, d: int, dev: int) -> Tuple[int, int, int]:
+    """A [n, heads, D] view with a unit inner stride -> (pointer, row stride, head stride)."""
+    strides = t.stride()
+    if t.shape != (n, heads, d) or strides[2] != 1 or t.get_device() != dev:
+        _bad(what, f"{name} {tuple(t.shape)} / {strides} on {t.device} is not [{n}, {heads}, {d}] with a "
+                   f"unit inner stride on the cache's device")
+    return t.data_ptr(), strides[0], strides[1]
 
 
-def _gpu(what: str, dev) -> None:
-    if dev.type != "cuda":
-        _bad(what, f"the tensors lie on {dev}: the kernels run on a GPU only")
+def _gpu(what: str, dev: int) -> None:
+    if dev < 0:
+        _bad(what, "the tensors are not on a GPU, and the kernels run nowhere else")
 
 
-def _launch(what: str, dev, fn, *args) -> None:
-    if dev.index is not None and dev.index != torch.cuda.current_device():
+def _launch(what: str, dev: int, fn, *args) -> None:
+    if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
     else:
         rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
     if rc:
-        raise RuntimeError(f"amdk8s_llm_{what} failed (rc={rc})")
+        raise RuntimeError(f"{what} failed (rc={rc})")
 
 
 def kv8_append(cache: Sequence[torch.Tensor], k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor,
@@ -166,39 +168,39 @@ def kv8_append(cache: Sequence[torch.Tensor], k: torch.Tensor, v: torch.Tensor, 
     appended position of a page is dead.  A page must be appended to by one sequence of a call only
     (shared prefix pages are for reading)."""
     what = "kv8_append"
-    dev, hkv, d, columns, pool = _pool(what, cache, pages)
-    n, s = k.shape[0], pages.shape[0]
-    kp = _rows(what, "k", k, hkv, d, dev)
-    vp = _rows(what, "v", v, hkv, d, dev)
-    if k.dtype not in _TYPES or v.dtype != k.dtype or v.shape[0] != n:
-        _bad(what, f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must have one shape and "
-                   f"one type of fp16, bf16, fp32")
+    dev, hkv, d, s, columns, pool = _pool(what, cache, pages)
+    kind = k.dtype
+    if kind not in _TYPES or v.dtype != kind:
+        _bad(what, f"k is {kind}, v {v.dtype}: one type of fp16, bf16, fp32")
+    n = k.shape[0]
+    kp, vp = _rows(what, "k", k, n, hkv, d, dev), _rows(what, "v", v, n, hkv, d, dev)
     starts, cus = _ints(what, "start", start, s, dev), _ints(what, "cu", cu, s + 1, dev)
     if (cos_t is None) != (sin_t is None) or (q is None) != (q_out is None):
         _bad(what, "cos_t goes with sin_t, and q with q_out")
-    tables = (None, None, 0)
+    turn = _NONE
     if cos_t is not None:
-        for t in (cos_t, sin_t):
-            if t.dtype != _F32 or t.dim() != 2 or t.shape[1] != d // 2 or t.shape[0] < columns * PAGE \
-                    or not t.is_contiguous() or t.device != dev or t.data_ptr() % 16:
-                _bad(what, f"rotation tables must be contiguous fp32 [>= {columns * PAGE}, {d // 2}] on "
-                           f"{dev}, 16-byte aligned")
-        tables = (cos_t.data_ptr(), sin_t.data_ptr(), min(cos_t.shape[0], sin_t.shape[0]))
-    qp = op = (None, 0, 0)
-    heads, otype = 0, _TYPES[k.dtype] if k.dtype != _F32 else 0
+        size = cos_t.shape
+        if len(size) != 2 or size[0] < columns * PAGE or size[1] != d // 2 or sin_t.shape != size \
+                or cos_t.dtype != _F32 or sin_t.dtype != _F32 or not cos_t.is_contiguous() \
+                or not sin_t.is_contiguous() or cos_t.get_device() != dev or sin_t.get_device() != dev:
+            _bad(what, f"rotation tables must be contiguous fp32 [>= {columns * PAGE}, {d // 2}] on the "
+                       f"cache's device")
+        turn = (cos_t.data_ptr(), sin_t.data_ptr(), size[0])
+        if (turn[0] | turn[1]) & 15:
+            _bad(what, "rotation tables must be 16-byte aligned")
+    qp = op = _NONE
+    heads, otype = 0, kind
     if q is not None:
-        heads = q.shape[1] if q.dim() == 3 else 0
-        qp, op = _rows(what, "q", q, heads, d, dev), _rows(what, "q_out", q_out, heads, d, dev)
-        if q.dtype != k.dtype or q.shape[0] != n or q_out.shape[0] != n or heads < 1 \
-                or q_out.dtype not in (torch.float16, torch.bfloat16) or (q.dtype != _F32 and q_out.dtype != q.dtype):
-            _bad(what, f"q {tuple(q.shape)} {q.dtype} / q_out {tuple(q_out.shape)} {q_out.dtype} must have "
-                       f"k's rows and type, q_out 16 bits")
-        otype = _TYPES[q_out.dtype]
+        heads, otype = q.shape[1], q_out.dtype
+        if q.dtype != kind or otype not in _QTYPES or (kind != _F32 and otype != kind):
+            _bad(what, f"q is {q.dtype}, q_out {otype}: q of k's type ({kind}), q_out the same, or fp16 or "
+                       f"bf16 for fp32")
+        qp, op = _rows(what, "q", q, n, heads, d, dev), _rows(what, "q_out", q_out, n, heads, d, dev)
     _gpu(what, dev)
-    if n == 0:
-        return
-    _launch(what, dev, _lib().amdk8s_llm_kv8_append, *pool, starts, cus, s, n, *kp, *vp, *qp, *op, heads,
-            *tables, _TYPES[k.dtype], otype)
+    if n:
+        _launch(what, dev, _lib().amdk8s_llm_kv8_append,
+                _APPEND.pack(*pool, starts, cus, s, n, *kp, *vp, *qp, *op, heads, *turn, _TYPES[kind],
+                             _QTYPES.get(otype, 0)))
 
 
 def kv8_read(cache: Sequence[torch.Tensor], pages: torch.Tensor, start: torch.Tensor, cu: torch.Tensor,
@@ -207,38 +209,49 @@ def kv8_read(cache: Sequence[torch.Tensor], pages: torch.Tensor, start: torch.Te
     ``k_out`` / ``v_out`` [N, Hkv, D] (fp16, bf16 or fp32; bf16 and fp32 hold them exactly).  Positions of
     unmapped pages read as zeros."""
     what = "kv8_read"
-    dev, hkv, d, _, pool = _pool(what, cache, pages)
-    n, s = k_out.shape[0], pages.shape[0]
-    kp, vp = _rows(what, "k_out", k_out, hkv, d, dev), _rows(what, "v_out", v_out, hkv, d, dev)
-    if k_out.dtype not in _TYPES or v_out.dtype != k_out.dtype or v_out.shape[0] != n:
-        _bad(what, f"k_out {tuple(k_out.shape)} {k_out.dtype} and v_out {tuple(v_out.shape)} {v_out.dtype} "
-                   f"must have one shape and one type of fp16, bf16, fp32")
+    dev, hkv, d, s, _, pool = _pool(what, cache, pages)
+    kind, n = k_out.dtype, k_out.shape[0]
+    if kind not in _TYPES or v_out.dtype != kind:
+        _bad(what, f"k_out is {kind}, v_out {v_out.dtype}: one type of fp16, bf16, fp32")
+    kp, vp = _rows(what, "k_out", k_out, n, hkv, d, dev), _rows(what, "v_out", v_out, n, hkv, d, dev)
     starts, cus = _ints(what, "start", start, s, dev), _ints(what, "cu", cu, s + 1, dev)
     _gpu(what, dev)
-    if n == 0:
-        return
-    _launch(what, dev, _lib().amdk8s_llm_kv8_read, *pool, starts, cus, s, n, *kp, *vp, _TYPES[k_out.dtype])
+    if n:
+        _launch(what, dev, _lib().amdk8s_llm_kv8_read,
+                _READ.pack(*pool, starts, cus, s, n, *kp, *vp, _TYPES[kind]))
 
 
 def _attention(what, q, out, hkv, d, dev, columns, span, window, sinks):
-    heads = q.shape[1] if q.dim() == 3 else 0
-    if heads < 1 or heads % hkv:
-        _bad(what, f"q {tuple(q.shape)}: heads must be a multiple of the cache's {hkv}")
-    qp = _rows(what, "q", q, heads, d, dev)
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        _bad(what, f"q is {q.dtype}: fp16 or bf16")
-    op = (None, 0, 0)
+    """Checked query and output rows -> (rows, heads, span, the record's fields of q, of out, type)."""
+    shape, kind = q.shape, q.dtype
+    if len(shape) != 3 or shape[1] < 1 or shape[1] % hkv:
+        _bad(what, f"q {tuple(shape)}: [rows, heads, D], heads a multiple of the cache's {hkv}")
+    if kind not in _QTYPES:
+        _bad(what, f"q is {kind}: fp16 or bf16")
+    n, heads, _ = shape
+    qp, op = _rows(what, "q", q, n, heads, d, dev), _NONE
     if out is not None:
-        op = _rows(what, "out", out, heads, d, dev)
-        if out.dtype != q.dtype or out.shape[0] != q.shape[0]:
-            _bad(what, f"out {tuple(out.shape)} {out.dtype} must have q's shape and type")
+        if out.dtype != kind:
+            _bad(what, f"out is {out.dtype}, q {kind}")
+        op = _rows(what, "out", out, n, heads, d, dev)
     most = columns * PAGE
-    span = most if span == 0 else span
+    span = span or most
     if not 0 < span <= most:
         _bad(what, f"span {span} is not in 1 .. {most} (the table's positions)")
     if not 0 <= window <= 1 << 30 or not 0 <= sinks <= 1 << 30:
         _bad(what, f"window {window} and sinks {sinks} must be in 0 .. 2^30")
-    return heads, qp, op, span
+    return n, heads, span, qp, op, _QTYPES[kind]
+
+
+def _attend(what, dev, size, run, record, scale) -> None:
+    need = size(record)
+    if need:
+        if need < 0:
+            raise RuntimeError(f"{what} failed (bad arguments)")
+        work = torch.empty(need, dtype=_F32, device=torch.device("cuda", dev))
+        _launch(what, dev, run, record, scale, work.data_ptr(), need)
+    else:
+        _launch(what, dev, run, record, scale, None, 0)
 
 
 def kv8_attn_decode(q: torch.Tensor, cache: Sequence[torch.Tensor], pages: torch.Tensor, pos: torch.Tensor,
@@ -253,33 +266,26 @@ def kv8_attn_decode(q: torch.Tensor, cache: Sequence[torch.Tensor], pages: torch
     [S, H D], a scale for each 32 and the scaled sum of each 16: the quantised GEMV's input); ``out`` may
     then be None. """
     what = "kv8_attn_decode"
-    dev, hkv, d, columns, pool = _pool(what, cache, pages)
-    heads, qp, op, span = _attention(what, q, out, hkv, d, dev, columns, span, window, sinks)
-    s = q.shape[0]
-    if pages.shape[0] != s:
-        _bad(what, f"{s} rows of q, {pages.shape[0]} of the page table")
-    if s > 65535:
-        _bad(what, f"{s} sequences: at most 65535 in a call")
+    dev, hkv, d, s, columns, pool = _pool(what, cache, pages)
+    n, heads, span, qp, op, kind = _attention(what, q, out, hkv, d, dev, columns, span, window, sinks)
+    if n != s or s > 65535:
+        _bad(what, f"{n} rows of q, {s} of the page table: as many, and at most 65535")
     at = _ints(what, "pos", pos, s, dev)
-    q8 = (None, None, None)
+    q8 = _NONE
     if q8_out is not None:
         x8, dx, sx = q8_out
         k = heads * d
         for t, dt, m in ((x8, torch.int8, k), (dx, _F32, k // 32), (sx, _F32, k // 16)):
-            if t.dtype != dt or t.shape != (s, m) or not t.is_contiguous() or t.device != dev:
+            if t.dtype != dt or t.shape != (s, m) or not t.is_contiguous() or t.get_device() != dev:
                 _bad(what, f"q8_out must be contiguous int8 [{s}, {k}], fp32 [{s}, {k // 32}] and fp32 "
                            f"[{s}, {k // 16}]")
         q8 = (x8.data_ptr(), dx.data_ptr(), sx.data_ptr())
     elif out is None:
         _bad(what, "neither out nor q8_out")
     _gpu(what, dev)
-    if s == 0:
-        return
     lib = _lib()
-    need = lib.amdk8s_llm_kv8_decode_work(s, heads, hkv, d, span, window, sinks, q8_out is not None)
-    work = torch.empty(need, dtype=_F32, device=dev) if need else None
-    _launch(what, dev, lib.amdk8s_llm_kv8_decode, *pool, *qp, at, s, heads, span, window, sinks, float(scale),
-            *op, _TYPES[q.dtype], *q8, work.data_ptr() if need else None, need)
+    _attend(what, dev, lib.amdk8s_llm_kv8_decode_work, lib.amdk8s_llm_kv8_decode,
+            _ATTN.pack(*pool, at, 0, s, s, *qp, *op, heads, span, window, sinks, kind, *q8), scale)
 
 
 def kv8_attn_prompt(q: torch.Tensor, cache: Sequence[torch.Tensor], pages: torch.Tensor, start: torch.Tensor,
@@ -289,17 +295,15 @@ def kv8_attn_prompt(q: torch.Tensor, cache: Sequence[torch.Tensor], pages: torch
     row and head strides) is position ``start[s] + i`` of sequence s; its chunk's keys are in the cache
     already (:func:`kv8_append`).  ``span`` as for :func:`kv8_attn_decode`."""
     what = "kv8_attn_prompt"
-    dev, hkv, d, columns, pool = _pool(what, cache, pages)
-    heads, qp, op, span = _attention(what, q, out, hkv, d, dev, columns, span, window, sinks)
-    n, s = q.shape[0], pages.shape[0]
+    dev, hkv, d, s, columns, pool = _pool(what, cache, pages)
+    n, heads, span, qp, op, kind = _attention(what, q, out, hkv, d, dev, columns, span, window, sinks)
+    if out is None:
+        _bad(what, "no out")
     starts, cus = _ints(what, "start", start, s, dev), _ints(what, "cu", cu, s + 1, dev)
     if n * heads > 1 << 30:
         _bad(what, f"{n} rows x {heads} heads: at most 2^30 in a call")
     _gpu(what, dev)
-    if n == 0:
-        return
-    lib = _lib()
-    need = lib.amdk8s_llm_kv8_prompt_work(n, s, heads, hkv, d, span, window, sinks)
-    work = torch.empty(need, dtype=_F32, device=dev) if need else None
-    _launch(what, dev, lib.amdk8s_llm_kv8_prompt, *pool, starts, cus, s, n, *qp, heads, span, window, sinks,
-            float(scale), *op, _TYPES[q.dtype], work.data_ptr() if need else None, need)
+    if n:
+        lib = _lib()
+        _attend(what, dev, lib.amdk8s_llm_kv8_prompt_work, lib.amdk8s_llm_kv8_prompt,
+                _ATTN.pack(*pool, starts, cus, s, n, *qp, *op, heads, span, window, sinks, kind, 0, 0, 0), scale)

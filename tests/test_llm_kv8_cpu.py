@@ -69,7 +69,7 @@ OWN = {
     "append": [
         (with_arg("k", lambda t: t.double()), "type"),
         (with_arg("k", lambda t: t[:, :1]), "k "),
-        (with_arg("k", lambda t: t[:-1]), "one shape"),
+        (with_arg("k", lambda t: t[:-1]), "v "),
         (with_arg("v", lambda t: t.bfloat16()), "type"),
         (with_arg("v", lambda t: torch.zeros(N, D, HKV, dtype=t.dtype).transpose(1, 2)), "v "),
         (with_arg("start", lambda t: t.long()), "start"),
@@ -82,11 +82,11 @@ OWN = {
         (with_arg("q_out", lambda t: t.bfloat16()), "q_out"),
         (with_arg("q_out", lambda t: t.float()), "q_out"),
         (with_arg("q", lambda t: t.float()), "type"),
-        (with_arg("q", lambda t: t[:-1]), "rows"),
+        (with_arg("q", lambda t: t[:-1]), "q "),
     ],
     "read": [
         (with_arg("k_out", lambda t: t.double()), "type"),
-        (with_arg("v_out", lambda t: t[:-1]), "one shape"),
+        (with_arg("v_out", lambda t: t[:-1]), "v_out"),
         (with_arg("cu", lambda t: t.float()), "cu"),
     ],
     "decode": [
@@ -109,6 +109,7 @@ OWN = {
         (with_arg("out", lambda t: t[:-1]), "out"),
         (with_arg("start", lambda t: t[:1]), "start"),
         (with_arg("cu", lambda t: t[:2]), "cu"),
+        (with_arg("out", None), "out"),
         (with_arg("span", 1000), "span"),
     ],
 }
