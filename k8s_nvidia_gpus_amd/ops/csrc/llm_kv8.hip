@@ -532,14 +532,20 @@ __device__ __forceinline__ float xor32(float x) {
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// Factor of a page's raw scores (codes x fitted query) to log2 units, ks the page's key scale and c the
+// query's own (>= 0).  Never 0: a masked score is -inf, and 0 x -inf would be NaN; the raw scores of a
+// zero page are 0, whatever the factor.  NaN stays.
+__device__ __forceinline__ float score_factor(float ks, float c) {
+  const float f = ks * c;
+  return f < 1e-37f ? 1e-37f : f;
+}
 // log2 of a page's value scale over the reference `vref` (the largest so far, > 0 unless all were 0).
 // The weights p = 2^(s - m) go to the matrix instruction as fp16 p vs / vref, so that pages of unlike
 // scales add up in one accumulator; the sum of the plain p's takes the factor back (`back`).  A zero
 // page has zero codes: any weight will do.  A NaN scale stays.  What the rounding costs: 2^-12 of a
 // weight, and weights below 2^-24 (of the largest weight times the largest value scale) are lost.
 __device__ __forceinline__ float value_weight(float vs, float vref, float& back) {
-  if (vs == 0.f) { back = 1.f; return 0.f; }
-  float lw = __builtin_amdgcn_logf(vs / vref);
+  float lw = vs == 0.f ? 0.f : __builtin_amdgcn_logf(vs / vref);
   lw = lw < -60.f ? -60.f : lw;                          // no fp16 weight is left there anyway
   back = __builtin_amdgcn_exp2f(-lw);
   return lw;
@@ -564,7 +570,7 @@ struct AttnArgs {
   long sq_tok, sq_head, so_tok, so_head;
   int H, G, span, window, sinks, parts, units;
   int per;                 // decode: pages a wave (at most 64)
-  float c2;                // scale x log2(e)
+  float c2, sign;          // |scale| x log2(e), and its sign (goes into the query)
   bool wide_q, wide_o;
 };
 
@@ -641,6 +647,7 @@ __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a
       f = fit_f16(amax);
       qf /= f;
     }
+    f *= a.sign;
 #pragma unroll
     for (int h = 0; h < KH; ++h)
 #pragma unroll
@@ -678,10 +685,10 @@ __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a
       if (more) load_values(i + 1);
       continue;
     }
-    const float f = ks * qf;
-    float sc[16];
+    const float f = score_factor(ks, qf);
+    float sc[16];                                        // raw: times f in log2 units
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sc[e] = acc[e >> 2][e & 3] * f;
+    for (int e = 0; e < 16; ++e) sc[e] = acc[e >> 2][e & 3];
     const bool whole = base + kPage - 1 <= last &&
                        (a.window <= 0 || base > pos - a.window || base + kPage <= a.sinks);
     if (!whole) {                                        // a border inside the page (wave-uniform)
@@ -701,10 +708,13 @@ __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a
     float mx = sc[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+    mx *= f;
     if (vs > vref) {                                     // uniform
-      const float r = vref / vs;
+      if (vref > 0.f) {
+        const float r = vref / vs;
 #pragma unroll
-      for (int n = 0; n < ND; ++n) o[n] *= r;
+        for (int n = 0; n < ND; ++n) o[n] *= r;
+      }
       vref = vs;
     }
     // rescale only when the maximum rose by more than 2^8 somewhere: weights stay below 2^8
@@ -714,17 +724,19 @@ __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a
       const float mn = fmaxf(m, mx);
       const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
-      l *= al;
+      if (i) {
+        l *= al;
 #pragma unroll
-      for (int n = 0; n < ND; ++n) o[n] *= al;
+        for (int n = 0; n < ND; ++n) o[n] *= al;
+      }
     }
     float back;
     const float lw = value_weight(vs, vref, back) - (m == -INFINITY ? 0.f : m);
     h8 pa[2];
     float ls = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float p = sc[e] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sc[e] + lw);
+    for (int e = 0; e < 16; ++e) {                       // (a poisoned page: NaN, as for its whole row)
+      const float p = __builtin_amdgcn_exp2f(fmaf(sc[e], f, lw));
       ls += p;
       pa[e >> 3][e & 7] = (_Float16)p;
     }
@@ -938,6 +950,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
       f = fit_f16(amax);
       qf /= f;
     }
+    f *= a.sign;
 #pragma unroll
     for (int st = 0; st < KS; ++st)
 #pragma unroll
@@ -1027,11 +1040,8 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
           sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qa[st], sc[b], 0, 0, 0);
         }
       }
-      const float f = ks * qf;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sc[b][i] *= f;
+      const bool poisoned = ks != ks || vs != vs;
+      const float f = score_factor(poisoned ? 0.f : ks, qf);
       const bool whole = base + kPage - 1 <= w_lo && base + kPage <= end &&
                          (a.window <= 0 || base > w_hi - a.window || base + kPage <= a.sinks);
       if (!whole) {
@@ -1049,6 +1059,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
+      mx *= f;
       if (vs > vref) {
         const float q = vref / vs;
 #pragma unroll
@@ -1065,15 +1076,20 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
         for (int b = 0; b < DB; ++b) o[b] *= al;
       }
       float back;
-      const float lw = value_weight(vs, vref, back) - (m == -INFINITY ? 0.f : m);
+      const float lw = value_weight(poisoned ? 0.f : vs, vref, back) - (m == -INFINITY ? 0.f : m);
+      if (poisoned) {                                    // NaN for the rows that see a key of it
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[b][i] = sc[b][i] == -INFINITY ? -INFINITY : __builtin_nanf("");
+      }
       h8 pa[4];
       float ls = 0.f;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          // a NaN weight (a poisoned page) must not reach rows that do not see the key
-          const float p = !whole && sc[b][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sc[b][i] + lw);
+          const float p = __builtin_amdgcn_exp2f(fmaf(sc[b][i], f, lw));
           ls += p;
           pa[2 * b + (i >> 3)][i & 7] = (_Float16)p;
         }
@@ -1208,7 +1224,8 @@ AttnArgs make_attn(const AttnCall& c, float scale, void* work, long parts) {
   a.sq_tok = c.q.tok; a.sq_head = c.q.head; a.so_tok = c.out.tok; a.so_head = c.out.head;
   a.H = (int)c.heads; a.G = (int)(c.heads / c.c.hkv);
   a.span = (int)c.span; a.window = (int)c.window; a.sinks = (int)c.sinks; a.parts = (int)parts;
-  a.c2 = scale * 1.4426950408889634f;
+  a.c2 = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
+  a.sign = scale < 0.f ? -1.f : 1.f;
   a.wide_q = wide16(c.q, 2);
   a.wide_o = c.out.at && wide16(c.out, 2);
   return a;

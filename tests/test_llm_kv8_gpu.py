@@ -245,6 +245,20 @@ def test_decode_large_and_small_queries(KV):
             check(out[s:s + 1], reference(cache, rows[s], q[s:s + 1], n - 1, 0.1 / size))
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1e-20])
+def test_scales_of_any_sign(KV, scale):
+    cache, rows, q = prompt_case(KV, [0, 130], [100, 40], 8, 2, 128, "int8", torch.float16, seed=18)
+    cache.ks[rows[0][0]] = 0.0
+    bits(cache.k)[rows[0][0]] = 0
+    out = torch.empty_like(q)
+    KV.kv8_attn_prompt(q, cache, ints(rows), ints([0, 130]), ints([0, 100, 140]), out, scale)
+    check(out[:100], reference(cache, rows[0], q[:100], 0, scale))
+    check(out[100:], reference(cache, rows[1], q[100:], 130, scale))
+    KV.kv8_attn_decode(q[:2], cache, ints(rows), ints([99, 169]), out[:2], scale)
+    for s, p in enumerate((99, 169)):
+        check(out[s:s + 1], reference(cache, rows[s], q[s:s + 1], p, scale))
+
+
 def test_decode_a_poisoned_page_poisons_those_that_see_it(KV):
     cache, rows, q, pos = decode_case(KV, [300, 300, 300], 8, 2, 128, "int8", torch.float16, seed=11)
     cache.vs[rows[0][2], 1] = float("nan")
