@@ -543,7 +543,10 @@ __device__ __forceinline__ float score_factor(float ks, float c) {
 // The weights p = 2^(s - m) go to the matrix instruction as fp16 p vs / vref, so that pages of unlike
 // scales add up in one accumulator; the sum of the plain p's takes the factor back (`back`).  A zero
 // page has zero codes: any weight will do.  A NaN scale stays.  What the rounding costs: 2^-12 of a
-// weight, and weights below 2^-24 (of the largest weight times the largest value scale) are lost.
+// weight, and weights below 2^-32 (of the largest weight times the largest value scale) are lost.
+// The reference maximum lies up to 8 below the true one (rescaling is put off that long) and kBias above
+// the exponent's: weights reach from 2^15, under fp16's largest, down to 2^-31 of the largest's step.
+constexpr float kDefer = 8.f, kBias = 7.f;
 __device__ __forceinline__ float value_weight(float vs, float vref, float& back) {
   float lw = vs == 0.f ? 0.f : __builtin_amdgcn_logf(vs / vref);
   lw = lw < -60.f ? -60.f : lw;                          // no fp16 weight is left there anyway
@@ -717,8 +720,8 @@ __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a
       }
       vref = vs;
     }
-    // rescale only when the maximum rose by more than 2^8 somewhere: weights stay below 2^8
-    if (__ballot(mx > m + 8.f) != 0) {
+    // rescale only when the maximum rose by more than 2^kDefer somewhere
+    if (__ballot(mx > m + kDefer) != 0) {
       mx = fmaxf(mx, xor16(mx));
       mx = fmaxf(mx, xor32(mx));
       const float mn = fmaxf(m, mx);
@@ -731,7 +734,7 @@ __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a
       }
     }
     float back;
-    const float lw = value_weight(vs, vref, back) - (m == -INFINITY ? 0.f : m);
+    const float lw = value_weight(vs, vref, back) + (m == -INFINITY ? kBias : kBias - m);
     h8 pa[2];
     float ls = 0.f;
 #pragma unroll
@@ -899,10 +902,17 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
 // registers of a lane are, in order, the P operand's consecutive positions: P never moves.
 __device__ __forceinline__ int swap23(int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); }
 
+// LDS images in 16-byte chunks: chunk ch of a key row (even ones first, so that a thread's two halves of
+// 16 codes do not meet the next thread's in a bank) and of a value row, XORed by the row
+template <int D>
+__device__ __forceinline__ int key_chunk(int row, int ch) {
+  return (ch >> 1 | (ch & 1) * (D / 16)) ^ (row & (D / 8 - 1));
+}
+__device__ __forceinline__ int value_chunk(int d, int ch) { return ch ^ (d & 7); }
+
 template <int D, bool FP8, int T, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a) {
   constexpr int NT = 64 * NW, RB = 2 * D, KT = kPage * RB, BUF = 2 * KT;    // bytes: key row, tile, K + V
-  constexpr int KC = RB / 16 - 1;                        // swizzle mask of a key row's 16-byte chunks
   constexpr int NCH = kPage * D / 16, CH = (NCH + NT - 1) / NT;             // 16-code chunks a thread
   constexpr int KS = D / 16, DB = D / 32;
   __shared__ __align__(16) char lds[2 * BUF];
@@ -964,7 +974,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
     for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
 
   uint4 kr[CH], vr[CH];
-  auto load_tile = [&](int id, int base) __attribute__((always_inline)) {
+  auto load_tile = [&](int id) __attribute__((always_inline)) {
     const long at = ((long)max(id, 0) * a.c.Hkv + kh) * kPage * D;
 #pragma unroll
     for (int u = 0; u < CH; ++u) {
@@ -982,18 +992,21 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
     for (int u = 0; u < CH; ++u) {
       const int c = tid + u * NT;
       if (NCH % NT == 0 || c < NCH) {
-        const int p = c / (D / 16), ch = 2 * (c % (D / 16)), row = swap23(p);
-        *reinterpret_cast<h8*>(kl + row * RB + ((ch ^ (row & KC)) << 4)) = codes_h8<FP8>(kr[u].x, kr[u].y);
-        *reinterpret_cast<h8*>(kl + row * RB + (((ch + 1) ^ (row & KC)) << 4)) = codes_h8<FP8>(kr[u].z, kr[u].w);
+        const int row = swap23(c / (D / 16)), ch = 2 * (c % (D / 16));
+        char* kw = kl + row * RB;
+        *reinterpret_cast<h8*>(kw + 16 * key_chunk<D>(row, ch)) = codes_h8<FP8>(kr[u].x, kr[u].y);
+        *reinterpret_cast<h8*>(kw + 16 * key_chunk<D>(row, ch + 1)) = codes_h8<FP8>(kr[u].z, kr[u].w);
         const int d = c >> 2, vch = 2 * (c & 3);
-        uint32_t w[4] = {vr[u].x, vr[u].y, vr[u].z, vr[u].w};
         if (FP8 && base + kPage > end) {                 // codes never written may be NaN: 0 x NaN
+          uint32_t w[4] = {vr[u].x, vr[u].y, vr[u].z, vr[u].w};
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (base + 16 * (c & 3) + e >= end) w[e >> 2] &= ~(0xffu << (8 * (e & 3)));
+          vr[u] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        *reinterpret_cast<h8*>(vl + d * 128 + ((vch ^ (d & 7)) << 4)) = codes_h8<FP8>(w[0], w[1]);
-        *reinterpret_cast<h8*>(vl + d * 128 + (((vch + 1) ^ (d & 7)) << 4)) = codes_h8<FP8>(w[2], w[3]);
+        char* vw = vl + d * (2 * kPage);
+        *reinterpret_cast<h8*>(vw + 16 * value_chunk(d, vch)) = codes_h8<FP8>(vr[u].x, vr[u].y);
+        *reinterpret_cast<h8*>(vw + 16 * value_chunk(d, vch + 1)) = codes_h8<FP8>(vr[u].z, vr[u].w);
       }
     }
   };
@@ -1002,12 +1015,18 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
     ks = a.c.ks[sc];
     vs = a.c.vs[sc];
   };
+  // LDS offsets of this lane's fragments: the second 32 keys and the other dims are constants behind them
+  int koff[KS], voff[4];
+#pragma unroll
+  for (int st = 0; st < KS; ++st) koff[st] = r * RB + 16 * key_chunk<D>(r, 2 * st + hh);
+#pragma unroll
+  for (int st = 0; st < 4; ++st) voff[st] = KT + r * (2 * kPage) + 16 * value_chunk(r, 2 * st + hh);
 
   int id = -1, id1 = -1;
   float ks = 0.f, vs = 0.f;
   if (t0 < t1) {
     id = a.c.page(s, seen.page(t0));
-    load_tile(id, seen.page(t0) * kPage);
+    load_tile(id);
     scales(id, ks, vs);
     id1 = t0 + 1 < t1 ? a.c.page(s, seen.page(t0 + 1)) : -1;
     store_tile(0, seen.page(t0) * kPage);
@@ -1020,26 +1039,21 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
     float ks1 = 0.f, vs1 = 0.f;
     int id2 = -1;
     if (kt + 1 < t1) {
-      load_tile(id1, next);
+      load_tile(id1);
       scales(id1, ks1, vs1);
       if (kt + 2 < t1) id2 = a.c.page(s, seen.page(kt + 2));
     }
     const bool hidden = base > w_hi || (a.window > 0 && base + kPage - 1 <= w_lo - a.window && base >= a.sinks);
     if (wave_in && id >= 0 && !hidden) {
       const char* kl = lds + buf * BUF;
-      const char* vl = kl + KT;
       f16v sc[2];
+      const f16v zero = {};
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int st = 0; st < KS; ++st)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[b][i] = 0.f;
-        const int row = 32 * b + r;
-#pragma unroll
-        for (int st = 0; st < KS; ++st) {
-          const h8 kf = *reinterpret_cast<const h8*>(kl + row * RB + (((2 * st + hh) ^ (row & KC)) << 4));
-          sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qa[st], sc[b], 0, 0, 0);
-        }
-      }
+        for (int b = 0; b < 2; ++b)
+          sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8*>(kl + koff[st] + 32 * b * RB),
+                                                         qa[st], st ? sc[b] : zero, 0, 0, 0);
       const bool poisoned = ks != ks || vs != vs;
       const float f = score_factor(poisoned ? 0.f : ks, qf);
       const bool whole = base + kPage - 1 <= w_lo && base + kPage <= end &&
@@ -1066,7 +1080,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
         for (int b = 0; b < DB; ++b) o[b] *= q;
         vref = vs;
       }
-      if (__ballot(mx > m + 8.f) != 0) {
+      if (__ballot(mx > m + kDefer) != 0) {
         mx = fmaxf(mx, xor32(mx));
         const float mn = fmaxf(m, mx);
         const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -1076,7 +1090,7 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
         for (int b = 0; b < DB; ++b) o[b] *= al;
       }
       float back;
-      const float lw = value_weight(poisoned ? 0.f : vs, vref, back) - (m == -INFINITY ? 0.f : m);
+      const float lw = value_weight(poisoned ? 0.f : vs, vref, back) + (m == -INFINITY ? kBias : kBias - m);
       if (poisoned) {                                    // NaN for the rows that see a key of it
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -1084,24 +1098,25 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
           for (int i = 0; i < 16; ++i) sc[b][i] = sc[b][i] == -INFINITY ? -INFINITY : __builtin_nanf("");
       }
       h8 pa[4];
-      float ls = 0.f;
+      float ls0 = 0.f, ls1 = 0.f;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(sc[b][i], f, lw));
-          ls += p;
-          pa[2 * b + (i >> 3)][i & 7] = (_Float16)p;
+        for (int i = 0; i < 16; i += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[b][i], f, lw));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[b][i + 1], f, lw));
+          ls0 += p0;
+          ls1 += p1;
+          pa[2 * b + (i >> 3)][i & 7] = (_Float16)p0;
+          pa[2 * b + (i >> 3)][(i & 7) + 1] = (_Float16)p1;
         }
-      l += ls * back;
+      l += (ls0 + ls1) * back;
 #pragma unroll
       for (int st = 0; st < 4; ++st)
 #pragma unroll
-        for (int b = 0; b < DB; ++b) {
-          const int d = 32 * b + r;
-          const h8 vf = *reinterpret_cast<const h8*>(vl + d * 128 + (((2 * st + hh) ^ (d & 7)) << 4));
-          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pa[st], o[b], 0, 0, 0);
-        }
+        for (int b = 0; b < DB; ++b)
+          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+              *reinterpret_cast<const h8*>(kl + voff[st] + 32 * b * (2 * kPage)), pa[st], o[b], 0, 0, 0);
     }
     if (kt + 1 < t1) store_tile(buf ^ 1, next);
     id = id1; id1 = id2; ks = ks1; vs = vs1;

@@ -145,9 +145,9 @@ def _gpu(what: str, dev: int) -> None:
 def _launch(what: str, dev: int, fn, *args) -> None:
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         raise RuntimeError(f"{what} failed (rc={rc})")
 
