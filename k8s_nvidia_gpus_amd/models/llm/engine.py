@@ -18,7 +18,10 @@ kind of server (``server.py``).  Design points:
   SDPA, writing the KV cache.  Without it, prompts run through the decode kernels 4 tokens at a
   time (causality comes from each token's own length).
 * **KV cache**: fp16 ``[layers, slots, kv_heads, max_ctx, 128]`` — one contiguous slab per
-  sequence slot; the server maps requests to slots.
+  sequence slot; the server maps requests to slots.  ``kv_type="int8"`` / ``"e4m3"`` keeps it in 8
+  bits instead (``ops/llm_kv8.py``: pages of 64 positions, a scale for each page and head; a slot owns
+  consecutive pages of each layer's pool): half the memory, and half the bytes that a step at a long
+  context reads.
 
 On a CPU (tests) the same API runs the fp32 reference maths (dequantised weights, PyTorch ops);
 the GPU path is compared against it.
@@ -80,6 +83,18 @@ class StepBuffers:
     host_evt: torch.cuda.Event = None
     ids_host: List[torch.Tensor] = None   # two pinned [T] landing buffers of decode_greedy_async
     ids_flip: int = 0
+    # 8-bit cache only: rotated fp16 queries, each token's page-table row, and the step's runs of
+    # consecutive positions (first position, first row, page-table row of each)
+    q16: torch.Tensor = None
+    pages: torch.Tensor = None
+    each: torch.Tensor = None        # int32 [T + 1]: 0 .. T (every token its own run)
+    runs: torch.Tensor = None        # int32 [3, T + 1] of a step whose tokens share slots
+    runs_host: torch.Tensor = None
+    run_pages: torch.Tensor = None
+
+
+# element types of the 8-bit KV cache
+KV8_TYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 
 
 class GreedyStep:
@@ -101,7 +116,9 @@ class GreedyStep:
 
 class Engine:
     def __init__(self, weights: ModelWeights, max_ctx: int = 4096, slots: int = 4,
-                 dense: Optional[bool] = None, use_graphs: bool = True):
+                 dense: Optional[bool] = None, use_graphs: bool = True, kv_type: str = "f16"):
+        if kv_type != "f16" and kv_type not in KV8_TYPES:
+            raise ValueError(f"kv_type {kv_type!r}: f16, {', '.join(KV8_TYPES)}")
         self.w = weights
         self.cfg: LLMConfig = weights.cfg
         self.device = weights.out_norm.device
@@ -114,9 +131,23 @@ class Engine:
         if c.head_dim != 128 and self.gpu:
             raise ValueError(f"head_dim {c.head_dim}: the decode kernels are built for 128")
         self.kv_dtype = torch.float16 if self.gpu else torch.float32
-        shape = (c.layers, slots, c.kv_heads, self.max_ctx, c.head_dim)
-        self.k_cache = torch.zeros(shape, dtype=self.kv_dtype, device=self.device)
-        self.v_cache = torch.zeros(shape, dtype=self.kv_dtype, device=self.device)
+        # the 8-bit cache's kernels run on the GPU; the CPU reference maths rounds nothing
+        self.kv_type = kv_type
+        self.kv8 = None                  # 8-bit cache: one KV8Cache for each layer
+        if kv_type != "f16" and self.gpu:
+            from k8s_nvidia_gpus_amd.ops import llm_kv8 as KV
+
+            self.KV = KV
+            each = self.max_ctx // KV.PAGE               # max_ctx is a multiple of 256
+            self.kv8 = [KV.KV8Cache.empty(slots * each, c.kv_heads, c.head_dim, KV8_TYPES[kv_type],
+                                          self.device) for _ in range(c.layers)]
+            self.kv_pages = torch.arange(slots * each, dtype=torch.int32,
+                                         device=self.device).view(slots, each)
+            self.k_cache = self.v_cache = None
+        else:
+            shape = (c.layers, slots, c.kv_heads, self.max_ctx, c.head_dim)
+            self.k_cache = torch.zeros(shape, dtype=self.kv_dtype, device=self.device)
+            self.v_cache = torch.zeros(shape, dtype=self.kv_dtype, device=self.device)
         self.cos, self.sin = rope_tables(self.max_ctx, c.head_dim, c.rope_theta, self.device)
         self.dense = self.gpu if dense is None else dense
         self._dense_w: Optional[Dict[str, torch.Tensor]] = None
@@ -218,6 +249,47 @@ class Engine:
     def embed(self, tokens: torch.Tensor) -> torch.Tensor:
         return self.w.tok_embd.dequant(torch.float32, rows=tokens.to(self.device))
 
+    # ------------------------------------------------------------------ 8-bit cache
+    def _kv8_runs(self, runs: Sequence[Tuple[int, int, int]]) -> tuple:
+        """(slot, first position, tokens) of each run -> (page-table rows, start, cu) on the GPU."""
+        cu = [0]
+        for _, _, n in runs:
+            cu.append(cu[-1] + n)
+        meta = torch.tensor([st for _, st, _ in runs] + cu, dtype=torch.int32, device=self.device)
+        rows = self.kv_pages[torch.tensor([s for s, _, _ in runs], device=self.device)]
+        return rows, meta[:len(runs)], meta[len(runs):]
+
+    def _kv8_append(self, i: int, qkv: torch.Tensor, runs: tuple, qh: torch.Tensor) -> None:
+        """Rows q|k|v [P, (H + 2 Hkv) D] (bias included): keys (rotated) and values into layer i's cache,
+        rotated fp16 queries into ``qh`` [H, P, D]."""
+        c = self.cfg
+        x = qkv.view(qkv.shape[0], c.heads + 2 * c.kv_heads, c.head_dim)
+        self.KV.kv8_append(self.kv8[i], x[:, c.heads:c.heads + c.kv_heads], x[:, c.heads + c.kv_heads:],
+                           *runs, self.cos, self.sin, q=x[:, :c.heads], q_out=qh.transpose(0, 1))
+
+    def _kv8_span(self, end: int) -> int:
+        """The attention's key bound for sequences of up to ``end`` positions (whole pages)."""
+        return min(-(-end // self.KV.PAGE) * self.KV.PAGE, self.max_ctx)
+
+    def _kv_store(self, i: int, slot: int, start: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Rotated keys and values [Hkv, P, D] into layer i's cache (the PyTorch prompt path)."""
+        if self.kv8 is None:
+            end = start + k.shape[1]
+            self.k_cache[i, slot, :, start:end] = k.to(self.kv_dtype)
+            self.v_cache[i, slot, :, start:end] = v.to(self.kv_dtype)
+            return
+        self.KV.kv8_append(self.kv8[i], k.transpose(0, 1), v.transpose(0, 1),
+                           *self._kv8_runs([(slot, start, k.shape[1])]))
+
+    def _kv_load(self, i: int, slot: int, end: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values [Hkv, end, D] of layer i's first ``end`` positions, as the cache holds them."""
+        if self.kv8 is None:
+            return self.k_cache[i, slot, :, :end], self.v_cache[i, slot, :, :end]
+        c = self.cfg
+        out = torch.empty(2, end, c.kv_heads, c.head_dim, dtype=self.kv_dtype, device=self.device)
+        self.KV.kv8_read(self.kv8[i], *self._kv8_runs([(slot, 0, end)]), out[0], out[1])
+        return out[0].transpose(0, 1), out[1].transpose(0, 1)
+
     # ------------------------------------------------------------------ dense forward
     def _forward_dense(self, tokens: torch.Tensor, slot: int, start: int) -> torch.Tensor:
         """Prompt tokens [P] of one sequence at positions start..start+P-1 → last-position logits
@@ -246,10 +318,10 @@ class Engine:
             v = qkv[:, c.dim + c.kv_dim:].view(P, c.kv_heads, c.head_dim).transpose(0, 1)
             q = apply_rope(q, cos, sin)
             k = apply_rope(k, cos, sin)
-            self.k_cache[i, slot, :, start:end] = k.to(self.kv_dtype)
-            self.v_cache[i, slot, :, start:end] = v.to(self.kv_dtype)
-            kk = self.k_cache[i, slot, :, :end].to(dt).repeat_interleave(c.group, 0)
-            vv = self.v_cache[i, slot, :, :end].to(dt).repeat_interleave(c.group, 0)
+            self._kv_store(i, slot, start, k, v)
+            kk, vv = self._kv_load(i, slot, end)
+            kk = kk.to(dt).repeat_interleave(c.group, 0)
+            vv = vv.to(dt).repeat_interleave(c.group, 0)
             o = F.scaled_dot_product_attention(q.to(dt)[None], kk[None], vv[None],
                                                attn_mask=None if mask is None else mask[None, None])
             o = o[0].transpose(0, 1).reshape(P, c.dim)
@@ -304,15 +376,23 @@ class Engine:
         scale = 1.0 / math.sqrt(c.head_dim)
         layers = self.w.layers
         normed = False                 # xn already holds this layer's attn_norm output
+        runs = self._kv8_runs([(slot, start, P)]) if self.kv8 is not None else None
         for i, L in enumerate(layers):
             if not normed:
                 LK.rmsnorm_f16(x, L.attn_norm, c.eps, xn)
             normed = False
             qkv = mm(xn, W[f"{i}.qkv"], W[f"{i}.bqkv"])
-            LK.rope_kv_f16(qkv, self.cos, self.sin, start, c.heads, c.kv_heads, self.max_ctx, qh,
-                           self.k_cache[i, slot], self.v_cache[i, slot])
+            if runs is not None:
+                self._kv8_append(i, qkv, runs, qh)
+            else:
+                LK.rope_kv_f16(qkv, self.cos, self.sin, start, c.heads, c.kv_heads, self.max_ctx, qh,
+                               self.k_cache[i, slot], self.v_cache[i, slot])
             if native_attn:            # hand-written causal GQA kernel, K/V read in place
-                LK.prefill_attn(qh, self.k_cache[i, slot], self.v_cache[i, slot], oh, start, scale)
+                if runs is not None:
+                    self.KV.kv8_attn_prompt(qh.transpose(0, 1), self.kv8[i], *runs,
+                                            oh.transpose(0, 1), scale, span=self._kv8_span(end))
+                else:
+                    LK.prefill_attn(qh, self.k_cache[i, slot], self.v_cache[i, slot], oh, start, scale)
                 x = self._res_norm(mm_res, x, o, W[f"{i}.o"], L.ffn_norm, xn)
                 self._gate_up(mm, xn, W[f"{i}.gu"], t)
                 if i + 1 < len(layers):     # ffn_down's finalize also writes the next attn_norm
@@ -321,15 +401,14 @@ class Engine:
                 else:
                     x = mm_res(x, t, W[f"{i}.down"])
                 continue
+            kk, vv = self._kv_load(i, slot, end)
             if self.prefill_gqa:       # K/V read in place by SDPA's GQA path; causal flag from 0
                 o = F.scaled_dot_product_attention(
-                    qh[None], self.k_cache[i, slot, :, :end][None],
-                    self.v_cache[i, slot, :, :end][None],
+                    qh[None], kk[None], vv[None],
                     attn_mask=None if (mask is None or start == 0) else lowright,
                     is_causal=mask is not None and start == 0, enable_gqa=True)
             else:
-                kk = self.k_cache[i, slot, :, :end].repeat_interleave(c.group, 0)
-                vv = self.v_cache[i, slot, :, :end].repeat_interleave(c.group, 0)
+                kk, vv = kk.repeat_interleave(c.group, 0), vv.repeat_interleave(c.group, 0)
                 o = F.scaled_dot_product_attention(
                     qh[None], kk[None], vv[None],
                     attn_mask=None if mask is None else mask[None, None])
@@ -367,26 +446,40 @@ class Engine:
         t = torch.empty(P, c.ffn, dtype=dt, device=self.device)
         layers = self.w.layers
         normed = False                 # xn already holds this layer's attn_norm output
+        runs = None
+        if self.kv8 is not None:
+            runs = self._kv8_runs([(slot, st, n) for n, (_, slot, st) in zip(lens, segs)])
+            span = self._kv8_span(max(st + n for n, (_, _, st) in zip(lens, segs)))
         for i, L in enumerate(layers):
             if not normed:
                 LK.rmsnorm_f16(x, L.attn_norm, c.eps, xn)
             normed = False
             qkv = mm(xn, W[f"{i}.qkv"], W[f"{i}.bqkv"])
+            if runs is not None:           # all sequences in one launch each
+                self._kv8_append(i, qkv, runs, qh)
+                if self.prefill_attn_native:
+                    self.KV.kv8_attn_prompt(qh.transpose(0, 1), self.kv8[i], *runs,
+                                            o.view(P, c.heads, c.head_dim),
+                                            1.0 / math.sqrt(c.head_dim), span=span)
             for s, (_, slot, st) in enumerate(segs):
+                if runs is not None:
+                    break
                 a, b = offs[s], offs[s + 1]
                 LK.rope_kv_f16(qkv[a:b], self.cos, self.sin, st, c.heads, c.kv_heads,
                                self.max_ctx, qh[:, a:b], self.k_cache[i, slot], self.v_cache[i, slot])
             for s, (_, slot, st) in enumerate(segs):
                 a, b = offs[s], offs[s + 1]
                 n, end = b - a, st + b - a
+                if self.prefill_attn_native and runs is not None:
+                    break
                 if self.prefill_attn_native:
                     LK.prefill_attn(qh[:, a:b], self.k_cache[i, slot], self.v_cache[i, slot],
                                     o[a:b].view(n, c.heads, c.head_dim).transpose(0, 1), st,
                                     1.0 / math.sqrt(c.head_dim))
                     continue
+                kk, vv = self._kv_load(i, slot, end)
                 os_ = F.scaled_dot_product_attention(
-                    qh[None, :, a:b], self.k_cache[i, slot, :, :end][None],
-                    self.v_cache[i, slot, :, :end][None], attn_mask=lowright[s],
+                    qh[None, :, a:b], kk[None], vv[None], attn_mask=lowright[s],
                     is_causal=n > 1 and st == 0, enable_gqa=True)
                 o[a:b] = os_[0].transpose(0, 1).reshape(n, c.dim)
             x = self._res_norm(mm_res, x, o, W[f"{i}.o"], L.ffn_norm, xn)
@@ -447,6 +540,14 @@ class Engine:
                 po=torch.zeros(T, c.heads, nsplit, c.head_dim, **f32),
                 pml=torch.zeros(T, c.heads, nsplit, 2, **f32), t=torch.zeros(T, c.ffn, **f32),
                 logits=torch.zeros(T, c.vocab, **f32))
+            if self.kv8 is not None:
+                cols = self.kv_pages.shape[1]
+                b.q16 = torch.zeros(T, c.heads, c.head_dim, dtype=torch.float16, device=dev)
+                b.pages = torch.zeros(T, cols, dtype=torch.int32, device=dev)
+                b.each = torch.arange(T + 1, dtype=torch.int32, device=dev)
+                b.runs = torch.zeros(3, T + 1, dtype=torch.int32, device=dev)
+                b.runs_host = torch.zeros(3, T + 1, dtype=torch.int32).pin_memory()
+                b.run_pages = torch.zeros(T, cols, dtype=torch.int32, device=dev)
             self._bufs[T] = b
         return b
 
@@ -486,9 +587,19 @@ class Engine:
             LK.rmsnorm_q8(xf, norm_w, c.eps, *qd)
             return qd, {}
 
+        if self.kv8 is not None:
+            torch.index_select(self.kv_pages, 0, b.slot, out=b.pages)
+            runs = (b.pages, b.pos, b.each)
+            if not fused:                 # some tokens share a slot: runs of consecutive positions
+                torch.index_select(self.kv_pages, 0, b.runs[2, :b.T], out=b.run_pages)
+                runs = (b.run_pages, b.runs[0, :b.T], b.runs[1])
         for i, L in enumerate(self.w.layers):
             self._qkv(b, L, *act(b.h, L.attn_norm))
-            if fused:
+            if self.kv8 is not None:
+                self._kv8_append(i, b.qkv, runs, b.q16.transpose(0, 1))
+                self.KV.kv8_attn_decode(b.q16, self.kv8[i], b.pages, b.pos, None, scale, span=span,
+                                        q8_out=qd)
+            elif fused:
                 LK.attn_decode(None, b.pos, b.slot, self.k_cache[i], self.v_cache[i], c.heads,
                                c.kv_heads, c.head_dim, self.max_ctx, scale, b.po, b.pml, *qd,
                                span=span, qkv=b.qkv, cos_t=self.cos, sin_t=self.sin)
@@ -526,6 +637,21 @@ class Engine:
                      **pro)
             off += w.n
 
+    @staticmethod
+    def _runs_of(positions: Sequence[int], slots: Sequence[int]) -> torch.Tensor:
+        """int32 [3, T + 1]: first position, first row and slot of each run of consecutive positions of
+        one slot; empty runs behind the last.  A page of the 8-bit cache takes one run of a step, so a
+        slot's tokens must be one run."""
+        T = len(positions)
+        at = [i for i in range(T) if i == 0 or slots[i] != slots[i - 1]
+              or positions[i] != positions[i - 1] + 1]
+        if len({slots[i] for i in at}) != len(at):
+            raise ValueError("decode: with an 8-bit KV cache the tokens of one slot must be consecutive "
+                             "positions, next to each other")
+        pad = [0] * (T - len(at))
+        return torch.tensor([[positions[i] for i in at] + pad + [0], at + [T] * (T + 1 - len(at)),
+                             [slots[i] for i in at] + pad + [0]], dtype=torch.int32)
+
     def _decode_native(self, tokens: Optional[Sequence[int]], positions: Sequence[int],
                        slots: Sequence[int], greedy: bool = False) -> torch.Tensor:
         """``tokens`` None: the tokens are the previous greedy step's ids of this batch size,
@@ -545,11 +671,14 @@ class Engine:
             b.host.copy_(torch.tensor([list(tokens), list(positions), list(slots)],
                                       dtype=torch.int32))
             b.meta.copy_(b.host, non_blocking=True)
+        fused = len(set(slots)) == len(slots)
+        if self.kv8 is not None and not fused:
+            b.runs_host.copy_(self._runs_of(positions, slots))
+            b.runs.copy_(b.runs_host, non_blocking=True)
         if b.host_evt is None:
             b.host_evt = torch.cuda.Event()
         b.host_evt.record()
         span = self._span(max(positions))
-        fused = len(set(slots)) == len(slots)
 
         def step():
             self._step_kernels(b, span, fused)
@@ -733,7 +862,10 @@ class Engine:
                 slots = list(range(T)) if T <= self.slots else [0] * T
                 for span in spans:
                     for greedy in (False, True):
-                        self._decode_native([0] * T, [span - 1] * T, slots, greedy=greedy)
+                        at = [span - 1] * T
+                        if self.kv8 is not None and T > self.slots:   # one run of one slot
+                            at = list(range(span - T, span))
+                        self._decode_native([0] * T, at, slots, greedy=greedy)
         torch.cuda.synchronize(self.device)
 
 

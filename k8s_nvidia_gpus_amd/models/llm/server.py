@@ -64,7 +64,7 @@ from typing import Any, Dict, List, Optional
 
 import torch
 
-from .engine import Engine
+from .engine import KV8_TYPES, Engine
 from .sampling import SamplingParams, sample_token
 from .tokenizer import Tokenizer
 
@@ -1063,7 +1063,8 @@ def build_engine(args) -> tuple:
     if args.model:
         from .synthetic import load
 
-        eng, tok = load(args.model, device=device, max_ctx=args.ctx_size, slots=args.parallel)
+        eng, tok = load(args.model, device=device, max_ctx=args.ctx_size, slots=args.parallel,
+                        kv_type=args.cache_type)
         return eng, tok, os.path.basename(args.model)
     from .config import QWEN25_7B, tiny
     from .synthetic import write_synthetic_gguf, load
@@ -1074,11 +1075,12 @@ def build_engine(args) -> tuple:
         from .weights import ModelWeights
 
         w = ModelWeights.random(QWEN25_7B, device=device)
-        eng = Engine(w, max_ctx=args.ctx_size, slots=args.parallel)
+        eng = Engine(w, max_ctx=args.ctx_size, slots=args.parallel, kv_type=args.cache_type)
         return eng, Tokenizer.from_gguf(synthetic_vocab(QWEN25_7B.vocab)), "qwen2.5-7b-synthetic"
     path = os.path.join(tempfile.mkdtemp(prefix="amdk8s-llm-"), "tiny.gguf")
     write_synthetic_gguf(path, tiny())
-    eng, tok = load(path, device=device, max_ctx=args.ctx_size, slots=args.parallel)
+    eng, tok = load(path, device=device, max_ctx=args.ctx_size, slots=args.parallel,
+                    kv_type=args.cache_type)
     return eng, tok, "tiny-qwen2-synthetic"
 
 
@@ -1097,6 +1099,9 @@ def main(argv=None) -> int:
                     help="prompt tokens per chunk while other sequences decode (llama-server -ub)")
     ap.add_argument("-b", "--batch-size", type=int, default=2048,
                     help="prompt tokens per chunk while nothing decodes (llama-server -b)")
+    ap.add_argument("-ct", "--cache-type", choices=["f16", *KV8_TYPES], default="f16",
+                    help="KV cache elements: int8 and e4m3 (8 bits and a scale for each 64 positions "
+                         "and head) halve its memory and the bytes a step at a long context reads")
     ap.add_argument("-ngl", "--n-gpu-layers", type=int, default=999, help="accepted; all layers run on the GPU")
     ap.add_argument("-t", "--threads", type=int, default=0, help="accepted; the GPU does the work")
     ap.add_argument("--no-prompt-batch", action="store_true",

@@ -66,7 +66,7 @@ def write_synthetic_gguf(path: str, cfg: LLMConfig, seed: int = 0,
 
 
 def load(path: str, device="cuda", max_ctx: int = 4096, slots: int = 4,
-         dense: Optional[bool] = None):
+         dense: Optional[bool] = None, kv_type: str = "f16"):
     """GGUF file → (Engine, Tokenizer)."""
     from .engine import Engine
     from .tokenizer import Tokenizer
@@ -75,4 +75,4 @@ def load(path: str, device="cuda", max_ctx: int = 4096, slots: int = 4,
     with gguf.GGUFFile(path) as g:
         tok = Tokenizer.from_gguf(g.metadata)      # refuses unknown pre-tokenisers / bad templates
         w = ModelWeights.from_gguf(g, device=device)
-    return Engine(w, max_ctx=max_ctx, slots=slots, dense=dense), tok
+    return Engine(w, max_ctx=max_ctx, slots=slots, dense=dense, kv_type=kv_type), tok

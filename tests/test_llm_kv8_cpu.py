@@ -128,3 +128,46 @@ def test_wrong_arguments_are_refused(name, i):
 def test_a_cache_that_no_kernel_reads_is_refused(bad):
     with pytest.raises(ValueError, match="KV8Cache"):
         KV.KV8Cache.empty(**{**dict(pages=2, kv_heads=1, head_dim=64, dtype=torch.int8, device="cpu"), **bad})
+
+
+# ------------------------------------------------------------------------------------------- the engine
+@pytest.fixture(scope="module")
+def tiny_model(tmp_path_factory):
+    from k8s_nvidia_gpus_amd.models.llm import tiny
+    from k8s_nvidia_gpus_amd.models.llm.synthetic import write_synthetic_gguf
+
+    return write_synthetic_gguf(str(tmp_path_factory.mktemp("llm") / "tiny.gguf"), tiny())
+
+
+def test_engine_takes_the_cache_types_it_knows(tiny_model):
+    from k8s_nvidia_gpus_amd.models.llm.synthetic import load
+
+    with pytest.raises(ValueError, match="kv_type"):
+        load(tiny_model, device="cpu", max_ctx=256, kv_type="q4_0")
+    a, _ = load(tiny_model, device="cpu", max_ctx=256)
+    b, _ = load(tiny_model, device="cpu", max_ctx=256, kv_type="int8")   # the CPU reference maths
+    assert b.kv_type == "int8" and b.kv8 is None
+    assert torch.equal(a.prefill([5, 6, 7], 1), b.prefill([5, 6, 7], 1))
+    assert torch.equal(a.decode([9], [3], [1]), b.decode([9], [3], [1]))
+
+
+def test_engine_runs_of_a_step():
+    from k8s_nvidia_gpus_amd.models.llm.engine import Engine
+
+    assert Engine._runs_of([4, 5, 6], [2, 2, 2]).tolist() == [[4, 0, 0, 0], [0, 3, 3, 3], [2, 0, 0, 0]]
+    assert Engine._runs_of([9, 3, 4], [0, 1, 1]).tolist() == [[9, 3, 0, 0], [0, 1, 3, 3], [0, 1, 0, 0]]
+    for positions, slots in (([4, 4], [0, 0]), ([5, 4], [0, 0]), ([1, 7, 2], [0, 1, 0])):
+        with pytest.raises(ValueError, match="consecutive"):
+            Engine._runs_of(positions, slots)
+
+
+def test_server_passes_the_cache_type_on(tmp_path):
+    from types import SimpleNamespace
+
+    from k8s_nvidia_gpus_amd.models.llm import server
+
+    eng, _, _ = server.build_engine(SimpleNamespace(model=None, synthetic="tiny", ctx_size=256, parallel=2,
+                                                    cache_type="e4m3"))
+    assert eng.kv_type == "e4m3"
+    with pytest.raises(SystemExit):
+        server.main(["--cache-type", "fp4"])
