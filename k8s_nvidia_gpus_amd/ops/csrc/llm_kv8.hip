@@ -902,19 +902,48 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
 // registers of a lane are, in order, the P operand's consecutive positions: P never moves.
 __device__ __forceinline__ int swap23(int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); }
 
-// LDS images in 16-byte chunks: chunk ch of a key row (even ones first, so that a thread's two halves of
-// 16 codes do not meet the next thread's in a bank) and of a value row, XORed by the row
+// A tile's LDS image: key rows of 2 D bytes and value rows of 128 (64 positions of a dim) in fp16, each
+// row 16 bytes longer than its data, so that rows lie in banks of their own and a lane's fragments are
+// constants behind one address.  A key row has its even 16-byte chunks first (a thread stages chunks 2 c
+// and 2 c + 1: the next thread's do not meet them).
 template <int D>
-__device__ __forceinline__ int key_chunk(int row, int ch) {
-  return (ch >> 1 | (ch & 1) * (D / 16)) ^ (row & (D / 8 - 1));
+struct Image {
+  static constexpr int kKeyRow = 2 * D + 16, kValueRow = 2 * kPage + 16;
+  static constexpr int kKeys = kPage * kKeyRow, kValues = D * kValueRow;    // bytes, multiples of 1024
+  static __device__ __forceinline__ int key(int row, int ch) {
+    return row * kKeyRow + 16 * (ch >> 1 | (ch & 1) * (D / 16));
+  }
+  static __device__ __forceinline__ int value(int d, int ch) { return d * kValueRow + 16 * ch; }
+};
+
+// 16 key codes (chunk c of the page's) / 16 value codes into the image
+template <int D, bool FP8>
+__device__ __forceinline__ void image_keys(char* to, int c, const uint4& w) {
+  const int row = swap23(c / (D / 16)), ch = 2 * (c % (D / 16));
+  *reinterpret_cast<h8*>(to + Image<D>::key(row, ch)) = codes_h8<FP8>(w.x, w.y);
+  *reinterpret_cast<h8*>(to + Image<D>::key(row, ch + 1)) = codes_h8<FP8>(w.z, w.w);
 }
-__device__ __forceinline__ int value_chunk(int d, int ch) { return ch ^ (d & 7); }
+// codes of positions that were never written (`live` and up of the page's 64) may be NaN, and a weight of
+// 0 would not hide them
+template <int D, bool FP8>
+__device__ __forceinline__ void image_values(char* to, int c, const uint4& v, int live) {
+  const int d = c >> 2, ch = 2 * (c & 3);
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if (FP8 && live < kPage) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (8 * ch + e >= live) w[e >> 2] &= ~(0xffu << (8 * (e & 3)));
+  }
+  *reinterpret_cast<h8*>(to + Image<D>::value(d, ch)) = codes_h8<FP8>(w[0], w[1]);
+  *reinterpret_cast<h8*>(to + Image<D>::value(d, ch + 1)) = codes_h8<FP8>(w[2], w[3]);
+}
 
 template <int D, bool FP8, int T, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a) {
-  constexpr int NT = 64 * NW, RB = 2 * D, KT = kPage * RB, BUF = 2 * KT;    // bytes: key row, tile, K + V
-  constexpr int NCH = kPage * D / 16, CH = (NCH + NT - 1) / NT;             // 16-code chunks a thread
+  typedef Image<D> I;
   constexpr int KS = D / 16, DB = D / 32;
+  constexpr int NT = 64 * NW, NCH = kPage * D / 16, CH = (NCH + NT - 1) / NT;   // 16-code chunks a thread
+  constexpr int BUF = I::kKeys + I::kValues;
   __shared__ __align__(16) char lds[2 * BUF];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hh = lane >> 5;
@@ -985,87 +1014,86 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
       }
     }
   };
-  auto store_tile = [&](int buf, int base) __attribute__((always_inline)) {
-    char* kl = lds + buf * BUF;
-    char* vl = kl + KT;
+  auto store_tile = [&](int buf, int live) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < CH; ++u) {
       const int c = tid + u * NT;
       if (NCH % NT == 0 || c < NCH) {
-        const int row = swap23(c / (D / 16)), ch = 2 * (c % (D / 16));
-        char* kw = kl + row * RB;
-        *reinterpret_cast<h8*>(kw + 16 * key_chunk<D>(row, ch)) = codes_h8<FP8>(kr[u].x, kr[u].y);
-        *reinterpret_cast<h8*>(kw + 16 * key_chunk<D>(row, ch + 1)) = codes_h8<FP8>(kr[u].z, kr[u].w);
-        const int d = c >> 2, vch = 2 * (c & 3);
-        if (FP8 && base + kPage > end) {                 // codes never written may be NaN: 0 x NaN
-          uint32_t w[4] = {vr[u].x, vr[u].y, vr[u].z, vr[u].w};
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (base + 16 * (c & 3) + e >= end) w[e >> 2] &= ~(0xffu << (8 * (e & 3)));
-          vr[u] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        char* vw = vl + d * (2 * kPage);
-        *reinterpret_cast<h8*>(vw + 16 * value_chunk(d, vch)) = codes_h8<FP8>(vr[u].x, vr[u].y);
-        *reinterpret_cast<h8*>(vw + 16 * value_chunk(d, vch + 1)) = codes_h8<FP8>(vr[u].z, vr[u].w);
+        image_keys<D, FP8>(lds + buf * BUF, c, kr[u]);
+        image_values<D, FP8>(lds + buf * BUF + I::kKeys, c, vr[u], live);
       }
     }
   };
-  auto scales = [&](int id, float& ks, float& vs) __attribute__((always_inline)) {
-    const long sc = (long)max(id, 0) * a.c.Hkv + kh;
-    ks = a.c.ks[sc];
-    vs = a.c.vs[sc];
+  // Table entries and scales of 64 pages at a time, a page a lane: a load for every page would have to be
+  // waited for with the tile's own loads, which are in the same queue.
+  int held = t0 - 64, my_id = -1;
+  float my_ks = 0.f, my_vs = 0.f;
+  auto entry = [&](int t, int& id, float& ks, float& vs) __attribute__((always_inline)) {
+    if (t >= held + 64) {                                // uniform; t only grows
+      held = t;
+      my_id = -1;
+      if (t + lane < t1) {
+        my_id = a.c.page(s, seen.page(t + lane));
+        const long sc = (long)max(my_id, 0) * a.c.Hkv + kh;
+        my_ks = a.c.ks[sc];
+        my_vs = a.c.vs[sc];
+      }
+    }
+    id = __builtin_amdgcn_readlane(my_id, t - held);
+    ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_ks), t - held));
+    vs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_vs), t - held));
   };
-  // LDS offsets of this lane's fragments: the second 32 keys and the other dims are constants behind them
-  int koff[KS], voff[4];
-#pragma unroll
-  for (int st = 0; st < KS; ++st) koff[st] = r * RB + 16 * key_chunk<D>(r, 2 * st + hh);
-#pragma unroll
-  for (int st = 0; st < 4; ++st) voff[st] = KT + r * (2 * kPage) + 16 * value_chunk(r, 2 * st + hh);
+  const int kfrag = I::key(r, hh), vfrag = I::kKeys + I::value(r, hh);
 
-  int id = -1, id1 = -1;
+  int id = -1;
   float ks = 0.f, vs = 0.f;
   if (t0 < t1) {
-    id = a.c.page(s, seen.page(t0));
+    entry(t0, id, ks, vs);
     load_tile(id);
-    scales(id, ks, vs);
-    id1 = t0 + 1 < t1 ? a.c.page(s, seen.page(t0 + 1)) : -1;
-    store_tile(0, seen.page(t0) * kPage);
+    store_tile(0, end - seen.page(t0) * kPage);
   }
   __syncthreads();
-  for (int kt = t0; kt < t1; ++kt) {
-    const int buf = (kt - t0) & 1;
-    const int base = seen.page(kt) * kPage;
-    const int next = kt + 1 < t1 ? seen.page(kt + 1) * kPage : 0;
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    const int base = seen.page(t) * kPage;
+    int id1 = -1;
     float ks1 = 0.f, vs1 = 0.f;
-    int id2 = -1;
-    if (kt + 1 < t1) {
+    if (t + 1 < t1) {
+      entry(t + 1, id1, ks1, vs1);
       load_tile(id1);
-      scales(id1, ks1, vs1);
-      if (kt + 2 < t1) id2 = a.c.page(s, seen.page(kt + 2));
     }
     const bool hidden = base > w_hi || (a.window > 0 && base + kPage - 1 <= w_lo - a.window && base >= a.sinks);
     if (wave_in && id >= 0 && !hidden) {
-      const char* kl = lds + buf * BUF;
+      const char* kl = lds + buf * BUF + kfrag;
       f16v sc[2];
       const f16v zero = {};
 #pragma unroll
       for (int st = 0; st < KS; ++st)
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8*>(kl + koff[st] + 32 * b * RB),
-                                                         qa[st], st ? sc[b] : zero, 0, 0, 0);
+          sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+              *reinterpret_cast<const h8*>(kl + 16 * st + 32 * b * I::kKeyRow), qa[st], st ? sc[b] : zero, 0, 0, 0);
+      // the order: two key fragments of either half read ahead of the matrix instructions that take them
+      constexpr int AHEAD = 2;
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);            // LDS reads
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        if (st + AHEAD < KS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);                  // matrix instructions
+      }
       const bool poisoned = ks != ks || vs != vs;
       const float f = score_factor(poisoned ? 0.f : ks, qf);
       const bool whole = base + kPage - 1 <= w_lo && base + kPage <= end &&
                          (a.window <= 0 || base > w_hi - a.window || base + kPage <= a.sinks);
       if (!whole) {
+        const int at = base + 8 * hh, hi = min(pos, end - 1) - at;          // of the registers' own offsets
+        const int lo = (a.window > 0 ? pos - a.window : -1) - at, sinks = a.sinks - at;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int j = base + 32 * b + 16 * (i >> 3) + 8 * hh + (i & 7);
-            const bool in = j <= pos && j < end && (a.window <= 0 || j > pos - a.window || j < a.sinks);
-            sc[b][i] = in ? sc[b][i] : -INFINITY;
+            const int x = 32 * b + 16 * (i >> 3) + (i & 7);
+            sc[b][i] = ((x <= hi) & ((x > lo) | (x < sinks))) ? sc[b][i] : -INFINITY;
           }
       }
       float mx = sc[0][0];
@@ -1090,36 +1118,45 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
         for (int b = 0; b < DB; ++b) o[b] *= al;
       }
       float back;
-      const float lw = value_weight(poisoned ? 0.f : vs, vref, back) + (m == -INFINITY ? kBias : kBias - m);
+      const float vw = value_weight(poisoned ? 0.f : vs, vref, back), up = m == -INFINITY ? kBias : kBias - m;
       if (poisoned) {                                    // NaN for the rows that see a key of it
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[b][i] = sc[b][i] == -INFINITY ? -INFINITY : __builtin_nanf("");
+          for (int i = 0; i < 16; ++i) sc[b][i] = sc[b][i] == -INFINITY ? sc[b][i] : __builtin_nanf("");
+      }
+      if (vw < -6.f) {                                   // fp16 weights of so small values would lose their sum
+        back = 0.f;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(fmaf(sc[b][i], f, up));
       }
       h8 pa[4];
+      const h2 one = {(_Float16)1.f, (_Float16)1.f};
       float ls0 = 0.f, ls1 = 0.f;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[b][i], f, lw));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[b][i + 1], f, lw));
-          ls0 += p0;
-          ls1 += p1;
-          pa[2 * b + (i >> 3)][i & 7] = (_Float16)p0;
-          pa[2 * b + (i >> 3)][(i & 7) + 1] = (_Float16)p1;
+          const h2 p = {(_Float16)__builtin_amdgcn_exp2f(fmaf(sc[b][i], f, vw + up)),
+                        (_Float16)__builtin_amdgcn_exp2f(fmaf(sc[b][i + 1], f, vw + up))};
+          float& ls = i & 2 ? ls1 : ls0;
+          ls = __builtin_amdgcn_fdot2(p, one, ls, false);
+          pa[2 * b + (i >> 3)][i & 7] = p[0];
+          pa[2 * b + (i >> 3)][(i & 7) + 1] = p[1];
         }
-      l += (ls0 + ls1) * back;
+      l = fmaf(ls0 + ls1, back, l);
 #pragma unroll
       for (int st = 0; st < 4; ++st)
 #pragma unroll
         for (int b = 0; b < DB; ++b)
           o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-              *reinterpret_cast<const h8*>(kl + voff[st] + 32 * b * (2 * kPage)), pa[st], o[b], 0, 0, 0);
+              *reinterpret_cast<const h8*>(lds + buf * BUF + vfrag + 32 * st + 32 * b * I::kValueRow), pa[st], o[b],
+              0, 0, 0);
     }
-    if (kt + 1 < t1) store_tile(buf ^ 1, next);
-    id = id1; id1 = id2; ks = ks1; vs = vs1;
+    if (t + 1 < t1) store_tile(buf ^ 1, end - seen.page(t + 1) * kPage);
+    id = id1; ks = ks1; vs = vs1;
     __syncthreads();
   }
   l += xor32(l);
@@ -1272,22 +1309,42 @@ DecodePlan decode_plan(const AttnCall& c) {
   return {4, (int)per, (n + 4 * per - 1) / (4 * per)};
 }
 
-constexpr int kPromptWaves = 4;
-constexpr long kPromptGrid = 512;                        // two workgroups on each of the 256 CUs
-
 struct PromptPlan {
+  int nw;
   long units, parts;
 };
-// Workgroups that share a row block's keys: as many as fill the chip when there are few row blocks, each
-// with at least 8 pages.
+// Waves a workgroup (4 or 8, of 32 rows each) and workgroups that share a row block's pages, by what they
+// take (microseconds, measured at D 128): a page costs a workgroup 1.5 alone on its CU and 2.05 beside
+// another (4 waves: two fit), 1.95 with 8 waves (one fits); partial outputs cost a join launch and their
+// bytes.  The time is the longest row block's or that of the rounds over the chip, whichever is more; a
+// causal chunk's own pages count half, as its row blocks see them on average.
+// Both sides: 2048 rows at 0 57 (4 waves) against 67 us, 4096 at 0 144 against 132, 512 at 16000 154
+// against 142; 16 rows at 500 in 1 part 20, in 4 15, 512 rows at 0 19 against 30.
 PromptPlan prompt_plan(const AttnCall& c) {
-  const long rows = 32 * kPromptWaves, G = c.heads / c.c.hkv;
-  long units = c.n * G / rows + c.s;
-  if (G <= rows && units > c.n) units = c.n;
-  long parts = kPromptGrid / (units * c.c.hkv);
-  const long most = most_seen(c, (rows + G - 1) / G + 1) / 8;
-  parts = parts > most ? most : parts;
-  return {units, parts < 1 ? 1 : parts};
+  const long G = c.heads / c.c.hkv;
+  PromptPlan best{4, 0, 1};
+  double least = 0;
+  for (int nw = 4; nw <= 8; nw += 4) {
+    const long rows = 32 * nw, slots = nw == 8 ? 256 : 512;
+    long units = c.n * G / rows + c.s;
+    if (G <= rows && units > c.n) units = c.n;
+    const long n = most_seen(c, (rows + G - 1) / G + 1);
+    const long own = c.n / (kPage * c.s);
+    const double mean = n - 0.5 * (own < n ? own : n);
+    const double bytes = 8.0 * c.n * c.heads * c.c.d;
+    for (long p = 1; p <= n && p <= 64; ++p) {
+      const long wgs = units * c.c.hkv * p;
+      const double crowd = (wgs * mean / n - 256) / 128;  // CUs with two workgroups: none to most
+      const double page = nw == 8 ? 1.95 : 1.5 + 0.55 * (crowd < 0 ? 0 : crowd > 1 ? 1 : crowd);
+      const double longest = (double)((n + p - 1) / p) * page, all = (double)((wgs + slots - 1) / slots) * mean / p * page;
+      const double t = (longest > all ? longest : all) + (p > 1 ? 3.5 + p * bytes / 3.5e6 : 0);
+      if (best.units == 0 || t < least) {
+        least = t;
+        best = {nw, units, p};
+      }
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -1422,9 +1479,13 @@ int amdk8s_llm_kv8_prompt(const void* call, float scale, void* work, long work_f
   return by_format(c.c, [&](auto d, auto f) -> int {
     constexpr int DD = decltype(d)::value;
     constexpr bool F8 = decltype(f)::value;
-    constexpr int NW = kPromptWaves;
-    if (c.type == kF16) hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kF16, NW>), grid, dim3(64 * NW), 0, st, a);
-    else hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kBF16, NW>), grid, dim3(64 * NW), 0, st, a);
+    auto go = [&](auto nw) {
+      constexpr int NW = decltype(nw)::value;
+      if (c.type == kF16) hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kF16, NW>), grid, dim3(64 * NW), 0, st, a);
+      else hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kBF16, NW>), grid, dim3(64 * NW), 0, st, a);
+    };
+    if (plan.nw == 8) go(std::integral_constant<int, 8>{});
+    else go(std::integral_constant<int, 4>{});
     if (need) {
       const dim3 rows((unsigned)c.heads, (unsigned)c.n);
       if (c.type == kF16) hipLaunchKernelGGL((kv8_join_kernel<DD, kF16, 1, false>), rows, dim3(64), 0, st, a);
