@@ -147,6 +147,16 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   return to_codes4<FP8>(x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio);
 }
 
+// four dwords as a 4 x 4 matrix of bytes, transposed
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  const uint32_t c = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
 // the least 2^e with amax <= qmax 2^e, from amax's bits (>= 0; NaN and infinity have the largest)
 template <bool FP8>
 __device__ __forceinline__ float block_scale(uint32_t bits) {
@@ -210,18 +220,22 @@ __device__ __forceinline__ bool find_piece(const Segs& sg, int unit, F count, Pi
   return false;
 }
 
-// The segment of row n (the whole wave asks for one row) and the row's position; false: in none.
-__device__ __forceinline__ bool find_row(const Segs& sg, int n, int& pos) {
+// The segment that row n is in (the whole wave asks for one row): its rows row .. end - 1, at pos ...
+struct Row {
+  int row, end, pos;
+};
+__device__ __forceinline__ bool find_row(const Segs& sg, int n, Row& out) {
   const int lane = threadIdx.x & 63;
   int s = 0;                                             // segments that end at or before row n
   for (int base = 0; base < sg.S; base += 64)
     s += __builtin_popcountll(__ballot(base + lane < sg.S && sg.cu[base + lane + 1] <= n));
   s = __builtin_amdgcn_readfirstlane(s);
+  out = Row{0, 0, 0};
   if (s >= sg.S) return false;
-  int row, cnt;
-  sg.get(s, row, cnt, pos);
-  pos += n - row;
-  return n >= row && n < row + cnt;
+  int cnt;
+  sg.get(s, out.row, cnt, out.pos);
+  out.end = out.row + cnt;
+  return n >= out.row && n < out.end;
 }
 
 __device__ __forceinline__ int pages_of(int n, int pos) { return (pos + n - 1) / kPage - pos / kPage + 1; }
@@ -257,7 +271,7 @@ struct AppendArgs {
   const float* cos_t;
   const float* sin_t;
   long sk_tok, sk_head, sv_tok, sv_head, sq_tok, sq_head, so_tok, so_head;
-  int H, units, table_rows;            // table_rows: rows of the rotation tables
+  int H, units, per, table_rows;       // per: query rows a wave; table_rows: rows of the rotation tables
   bool wide_kv, wide_q;
 };
 
@@ -273,26 +287,19 @@ __device__ __forceinline__ float turn_hi(float a, float b, float c, float s) {
   return x + y;
 }
 
-// eight pairs (d, d + D/2) of one row: rotated in fp32 with a rounding after every operation (one
-// definition of the rotated key's bits, whoever computes it)
+// eight pairs (d, d + D/2) of one row, and their rotation
 template <int T, int D>
-__device__ __forceinline__ void load_turned(const typename Elem<T>::type* row, bool wide, const float* cos_t,
-                                            const float* sin_t, long pos, int d0, float (&lo)[8], float (&hi)[8]) {
-  float a[8], b[8];
-  load_n<T, 8>(row + d0, wide, a);
-  load_n<T, 8>(row + D / 2 + d0, wide, b);
-  if (cos_t) {
-    float c[8], s[8];
-    load_n<kF32, 8>(cos_t + pos * (D / 2) + d0, true, c);
-    load_n<kF32, 8>(sin_t + pos * (D / 2) + d0, true, s);
+__device__ __forceinline__ void load_pairs(const typename Elem<T>::type* row, bool wide, int d0, float (&lo)[8],
+                                           float (&hi)[8]) {
+  load_n<T, 8>(row + d0, wide, lo);
+  load_n<T, 8>(row + D / 2 + d0, wide, hi);
+}
+__device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const float (&c)[8], const float (&s)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lo[i] = turn_lo(a[i], b[i], c[i], s[i]);
-      hi[i] = turn_hi(a[i], b[i], c[i], s[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { lo[i] = a[i]; hi[i] = b[i]; }
+  for (int i = 0; i < 8; ++i) {
+    const float a = lo[i], b = hi[i];
+    lo[i] = turn_lo(a, b, c[i], s[i]);
+    hi[i] = turn_hi(a, b, c[i], s[i]);
   }
 }
 
@@ -308,56 +315,73 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
   constexpr int PR = D / 16;                             // 8-pair items of a row
   constexpr int PER = kPage * PR / 256;                  // items a thread
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if ((int)blockIdx.x >= a.units * a.c.Hkv) {            // ---- queries
-    const int n = ((int)blockIdx.x - a.units * a.c.Hkv) * 4 + wave;
-    if (n >= a.sg.N) return;
-    int pos;
-    if (!find_row(a.sg, n, pos)) return;
-    if (pos >= a.table_rows) return;
-    const E* q = static_cast<const E*>(a.q) + (long)n * a.sq_tok;
+  if ((int)blockIdx.x >= a.units * a.c.Hkv) {            // ---- queries: a.per rows a wave
     typedef typename Elem<TO>::type EO;
-    EO* o = static_cast<EO*>(a.qo) + (long)n * a.so_tok;
-    for (int i = lane; i < a.H * PR; i += 64) {
-      const int h = i / PR, d0 = 8 * (i % PR);
-      float lo[8], hi[8];
-      load_turned<T, D>(q + h * a.sq_head, a.wide_q, a.cos_t, a.sin_t, pos, d0, lo, hi);
-      store_n<TO, 8>(o + h * a.so_head + d0, a.wide_q, lo);
-      store_n<TO, 8>(o + h * a.so_head + D / 2 + d0, a.wide_q, hi);
+    const int d0 = 8 * (lane % PR);                        // a lane's pairs, of every 64 / PR'th head
+    const int n0 = (((int)blockIdx.x - a.units * a.c.Hkv) * 4 + wave) * a.per;
+    Row at{0, 0, 0};
+    for (int n = n0; n < min(n0 + a.per, a.sg.N); ++n) {
+      if (n >= at.end && !find_row(a.sg, n, at)) continue;
+      const int pos = at.pos + n - at.row;
+      if (pos >= a.table_rows) continue;
+      const E* q = static_cast<const E*>(a.q) + (long)n * a.sq_tok;
+      EO* o = static_cast<EO*>(a.qo) + (long)n * a.so_tok;
+      float c[8], s[8];
+      if (a.cos_t) {
+        load_n<kF32, 8>(a.cos_t + (long)pos * (D / 2) + d0, true, c);
+        load_n<kF32, 8>(a.sin_t + (long)pos * (D / 2) + d0, true, s);
+      }
+#pragma unroll 4
+      for (int h = lane / PR; h < a.H; h += 64 / PR) {
+        float lo[8], hi[8];
+        load_pairs<T, D>(q + h * a.sq_head, a.wide_q, d0, lo, hi);
+        if (a.cos_t) turn(lo, hi, c, s);
+        store_n<TO, 8>(o + h * a.so_head + d0, a.wide_q, lo);
+        store_n<TO, 8>(o + h * a.so_head + D / 2 + d0, a.wide_q, hi);
+      }
     }
     return;
   }
   __shared__ uint32_t red[2][4];
-  __shared__ __align__(16) uint8_t img[kPage][D + 16];   // value codes by position
+  __shared__ __align__(8) uint8_t img[kPage][D + 8];     // value codes by position
   const int kh = blockIdx.x % a.c.Hkv;
   Piece pc;
   if (!find_piece(a.sg, blockIdx.x / a.c.Hkv, [](int n, int p) { return pages_of(n, p); }, pc)) return;
   const int pos = pc.pos, cnt = pc.cnt, row = pc.row;
   const int j = pos / kPage + pc.index;
-  const int id = a.c.page(pc.s, j);
-  if (id < 0) return;
+  if (j >= a.c.width) return;                            // behind the table (and its rotation tables)
   const int r0 = max(pos - j * kPage, 0), r1 = min(pos + cnt - j * kPage, kPage);   // new rows
   const long n0 = (long)row + j * kPage - pos;           // input row of the page's position 0
+  const E* kin = static_cast<const E*>(a.k) + kh * a.sk_head;
+  const E* vin = static_cast<const E*>(a.v) + kh * a.sv_head;
+  // the inputs do not wait for the table entry
+  float klo[PER][8] = {}, khi[PER][8] = {}, vlo[PER][8] = {}, vhi[PER][8] = {}, cs[PER][8] = {}, sn[PER][8] = {};
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int i = tid + 256 * u, r = i / PR, d0 = 8 * (i % PR);
+    if (r < r0 || r >= r1) continue;
+    load_pairs<T, D>(kin + (n0 + r) * a.sk_tok, a.wide_kv, d0, klo[u], khi[u]);
+    load_n<T, 8>(vin + (n0 + r) * a.sv_tok + 2 * d0, a.wide_kv, vlo[u]);
+    load_n<T, 8>(vin + (n0 + r) * a.sv_tok + 2 * d0 + 8, a.wide_kv, vhi[u]);
+    if (a.cos_t) {
+      load_n<kF32, 8>(a.cos_t + ((long)j * kPage + r) * (D / 2) + d0, true, cs[u]);
+      load_n<kF32, 8>(a.sin_t + ((long)j * kPage + r) * (D / 2) + d0, true, sn[u]);
+    }
+  }
+  const int id = a.c.page(pc.s, j);
+  if (id < 0) return;
   const long sc = (long)id * a.c.Hkv + kh;
   uint8_t* kc = a.c.k + sc * kPage * D;
   uint8_t* vc = a.c.v + sc * kPage * D;
   const float oldk = r0 ? a.c.ks[sc] : 0.f, oldv = r0 ? a.c.vs[sc] : 0.f;
-  const E* kin = static_cast<const E*>(a.k) + kh * a.sk_head;
-  const E* vin = static_cast<const E*>(a.v) + kh * a.sv_head;
-  float klo[PER][8], khi[PER][8], vlo[PER][8], vhi[PER][8];
   uint32_t mk = 0, mv = 0;                               // largest magnitudes, as bits (NaN largest)
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
-    const int i = tid + 256 * u, r = i / PR, d0 = 8 * (i % PR);
-    if (r >= r0 && r < r1) {
-      const long n = n0 + r;
-      load_turned<T, D>(kin + n * a.sk_tok, a.wide_kv, a.cos_t, a.sin_t, (long)j * kPage + r, d0, klo[u], khi[u]);
-      load_n<T, 8>(vin + n * a.sv_tok + 2 * d0, a.wide_kv, vlo[u]);
-      load_n<T, 8>(vin + n * a.sv_tok + 2 * d0 + 8, a.wide_kv, vhi[u]);
+    if (a.cos_t) turn(klo[u], khi[u], cs[u], sn[u]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        mk = max(mk, max(__float_as_uint(klo[u][e]) & 0x7fffffffu, __float_as_uint(khi[u][e]) & 0x7fffffffu));
-        mv = max(mv, max(__float_as_uint(vlo[u][e]) & 0x7fffffffu, __float_as_uint(vhi[u][e]) & 0x7fffffffu));
-      }
+    for (int e = 0; e < 8; ++e) {
+      mk = max(mk, max(__float_as_uint(klo[u][e]) & 0x7fffffffu, __float_as_uint(khi[u][e]) & 0x7fffffffu));
+      mv = max(mv, max(__float_as_uint(vlo[u][e]) & 0x7fffffffu, __float_as_uint(vhi[u][e]) & 0x7fffffffu));
     }
   }
 #pragma unroll
@@ -389,7 +413,6 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
   for (int u = 0; u < PER; ++u) {
     const int i = tid + 256 * u, r = i / PR, d0 = 8 * (i % PR);
     if (r >= r0 && r < r1) {
-      uint2 w;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         klo[u][e] = badk ? 0.f : klo[u][e] * ik;
@@ -397,43 +420,47 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
         vlo[u][e] = badv ? 0.f : vlo[u][e] * iv;
         vhi[u][e] = badv ? 0.f : vhi[u][e] * iv;
       }
-      w.x = to_codes4<FP8>(klo[u][0], klo[u][1], klo[u][2], klo[u][3]);
-      w.y = to_codes4<FP8>(klo[u][4], klo[u][5], klo[u][6], klo[u][7]);
-      *reinterpret_cast<uint2*>(kc + r * D + d0) = w;
-      w.x = to_codes4<FP8>(khi[u][0], khi[u][1], khi[u][2], khi[u][3]);
-      w.y = to_codes4<FP8>(khi[u][4], khi[u][5], khi[u][6], khi[u][7]);
-      *reinterpret_cast<uint2*>(kc + r * D + D / 2 + d0) = w;
-      uint4 x;
-      x.x = to_codes4<FP8>(vlo[u][0], vlo[u][1], vlo[u][2], vlo[u][3]);
-      x.y = to_codes4<FP8>(vlo[u][4], vlo[u][5], vlo[u][6], vlo[u][7]);
-      x.z = to_codes4<FP8>(vhi[u][0], vhi[u][1], vhi[u][2], vhi[u][3]);
-      x.w = to_codes4<FP8>(vhi[u][4], vhi[u][5], vhi[u][6], vhi[u][7]);
-      *reinterpret_cast<uint4*>(&img[r][2 * d0]) = x;
+      auto eight = [&](const float (&x)[8]) {
+        return make_uint2(to_codes4<FP8>(x[0], x[1], x[2], x[3]), to_codes4<FP8>(x[4], x[5], x[6], x[7]));
+      };
+      *reinterpret_cast<uint2*>(kc + r * D + d0) = eight(klo[u]);
+      *reinterpret_cast<uint2*>(kc + r * D + D / 2 + d0) = eight(khi[u]);
+      *reinterpret_cast<uint2*>(&img[r][2 * d0]) = eight(vlo[u]);
+      *reinterpret_cast<uint2*>(&img[r][2 * d0 + 8]) = eight(vhi[u]);
     }
   }
   __syncthreads();
+  // 8 positions of 4 dims a thread: eight lanes write a dim's 64 bytes
   const float rv = growv ? oldv * iv : 1.f;
-  for (int i = tid; i < D * 4; i += 256) {               // 16 positions of one dim
-    const int d = i % D, p0 = 16 * (i / D);
-    const bool has_new = p0 < r1 && p0 + 16 > r0;
-    if (!has_new && !(growv && p0 < r0)) continue;
-    uint4* at = reinterpret_cast<uint4*>(vc + d * kPage + p0);
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (p0 < r0 || p0 + 16 > r1) {                       // some of them are not new
-      const uint4 old = *at;
-      w[0] = old.x; w[1] = old.y; w[2] = old.z; w[3] = old.w;
-      if (growv) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = rescale4<FP8>(w[e], rv);
+  for (int u = 0; u < D * 2 / 256 + (D * 2 % 256 != 0); ++u) {
+    const int i = tid + 256 * u, p0 = 8 * (i & 7), d = 4 * (i >> 3);
+    const bool has_new = p0 < r1 && p0 + 8 > r0;
+    if (d >= D || (!has_new && !(growv && p0 < r0))) continue;
+    uint32_t lo[4], hi[4];                               // by position, then (transposed) by dim
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      lo[e] = *reinterpret_cast<const uint32_t*>(&img[p0 + e][d]);
+      hi[e] = *reinterpret_cast<const uint32_t*>(&img[p0 + 4 + e][d]);
+    }
+    transpose4(lo);
+    transpose4(hi);
+    uint32_t keep[2] = {0, 0};                           // bytes that are not new
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (p0 + e < r0 || p0 + e >= r1) keep[e >> 2] |= 0xffu << (8 * (e & 3));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint2* at = reinterpret_cast<uint2*>(vc + (d + e) * kPage + p0);
+      uint2 w = make_uint2(lo[e], hi[e]);
+      if (keep[0] | keep[1]) {
+        uint2 old = *at;
+        if (growv) { old.x = rescale4<FP8>(old.x, rv); old.y = rescale4<FP8>(old.y, rv); }
+        w.x = (w.x & ~keep[0]) | (old.x & keep[0]);
+        w.y = (w.y & ~keep[1]) | (old.y & keep[1]);
       }
+      *at = w;
     }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int r = p0 + e;
-      if (r >= r0 && r < r1)
-        w[e >> 2] = (w[e >> 2] & ~(0xffu << (8 * (e & 3)))) | ((uint32_t)img[r][d] << (8 * (e & 3)));
-    }
-    *at = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -451,7 +478,8 @@ struct ReadArgs {
 template <int D, bool FP8, int T>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
   typedef typename Elem<T>::type E;
-  __shared__ __align__(16) uint8_t img[kPage][D + 16];
+  __shared__ __align__(8) uint8_t img[kPage][D + 8];     // value codes by position
+  constexpr int PK = kPage * D / 16 / 256, PV = D * 2 / 256 + (D * 2 % 256 != 0);
   const int tid = threadIdx.x;
   const int kh = blockIdx.x % a.c.Hkv;
   Piece pc;
@@ -462,40 +490,61 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
   const long n0 = (long)row + j * kPage - pos;
   const int id = a.c.page(pc.s, j);
   const bool live = id >= 0;
-  const long sc = (long)max(id, 0) * a.c.Hkv + kh;
+  const long sc = (long)max(id, 0) * a.c.Hkv + kh;       // an unmapped page: page 0, times 0 (and no NaN code)
   const uint8_t* kc = a.c.k + sc * kPage * D;
   const uint8_t* vc = a.c.v + sc * kPage * D;
   const float sk = live ? a.c.ks[sc] : 0.f, sv = live ? a.c.vs[sc] : 0.f;
-  for (int i = tid; i < D * 4; i += 256) {               // 16 positions of one dim
-    const int d = i % D, p0 = 16 * (i / D);
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (live && p0 < r1 && p0 + 16 > r0) x = *reinterpret_cast<const uint4*>(vc + d * kPage + p0);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  const uint32_t mask = live ? ~0u : 0u;
+  uint4 kx[PK];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) img[p0 + e][d] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+  for (int u = 0; u < PK; ++u) kx[u] = reinterpret_cast<const uint4*>(kc)[tid + 256 * u];
+  uint2 vx[PV][4];                                       // 8 positions of 4 dims
+#pragma unroll
+  for (int u = 0; u < PV; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = tid + 256 * u, d = 4 * (i >> 3);
+      if (d < D) vx[u][e] = *reinterpret_cast<const uint2*>(vc + (d + e) * kPage + 8 * (i & 7));
+    }
+  auto put = [&](E* out, const uint32_t (&w)[4], float scale) __attribute__((always_inline)) {
+    float y[16], x[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      codes_f4<FP8>(w[c] & mask, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[4 * c + e] = x[e] * scale;
+    }
+    store_n<T, 16>(out, a.wide, y);
+  };
+#pragma unroll
+  for (int u = 0; u < PK; ++u) {
+    const int i = tid + 256 * u, r = i / (D / 16), d0 = 16 * (i % (D / 16));
+    const uint32_t w[4] = {kx[u].x, kx[u].y, kx[u].z, kx[u].w};
+    if (r >= r0 && r < r1) put(static_cast<E*>(a.ko) + (n0 + r) * a.sk_tok + kh * a.sk_head + d0, w, sk);
+  }
+#pragma unroll
+  for (int u = 0; u < PV; ++u) {
+    const int i = tid + 256 * u, p0 = 8 * (i & 7), d = 4 * (i >> 3);
+    if (d >= D) continue;
+    uint32_t lo[4], hi[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { lo[e] = vx[u][e].x; hi[e] = vx[u][e].y; }
+    transpose4(lo);
+    transpose4(hi);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      *reinterpret_cast<uint32_t*>(&img[p0 + e][d]) = lo[e];
+      *reinterpret_cast<uint32_t*>(&img[p0 + 4 + e][d]) = hi[e];
+    }
   }
   __syncthreads();
-  for (int i = tid; i < kPage * (D / 16); i += 256) {
-    const int r = i / (D / 16), d0 = 16 * (i % (D / 16));
+#pragma unroll
+  for (int u = 0; u < PK; ++u) {
+    const int i = tid + 256 * u, r = i / (D / 16), d0 = 16 * (i % (D / 16));
     if (r < r0 || r >= r1) continue;
-    const uint4 kx = live ? *reinterpret_cast<const uint4*>(kc + r * D + d0) : make_uint4(0, 0, 0, 0);
-    const uint4 vx = *reinterpret_cast<const uint4*>(&img[r][d0]);
-    float y[16], x[4];
-    const uint32_t kw[4] = {kx.x, kx.y, kx.z, kx.w}, vw[4] = {vx.x, vx.y, vx.z, vx.w};
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      codes_f4<FP8>(kw[c], x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[4 * c + e] = x[e] * sk;
-    }
-    store_n<T, 16>(static_cast<E*>(a.ko) + (n0 + r) * a.sk_tok + kh * a.sk_head + d0, a.wide, y);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      codes_f4<FP8>(vw[c], x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[4 * c + e] = x[e] * sv;
-    }
-    store_n<T, 16>(static_cast<E*>(a.vo) + (n0 + r) * a.sv_tok + kh * a.sv_head + d0, a.wide, y);
+    const uint2 a0 = *reinterpret_cast<const uint2*>(&img[r][d0]), a1 = *reinterpret_cast<const uint2*>(&img[r][d0 + 8]);
+    const uint32_t w[4] = {a0.x, a0.y, a1.x, a1.y};
+    put(static_cast<E*>(a.vo) + (n0 + r) * a.sv_tok + kh * a.sv_head + d0, w, sv);
   }
 }
 
@@ -806,8 +855,8 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = blockIdx.x, t = blockIdx.y, np = a.parts;
   if (!DECODE) {
-    int pos;
-    if (!find_row(a.sg, t, pos)) return;                 // no partials: the output row stays
+    Row at;
+    if (!find_row(a.sg, t, at)) return;                  // no partials: the output row stays
   }
   const long row = (long)t * a.H + h, step = (long)a.sg.N * a.H;
   float M = -INFINITY, L = 0.f;
@@ -1375,7 +1424,10 @@ int amdk8s_llm_kv8_append(const void* call, void* stream) {
   a.wide_kv = wide16(c.k, es) && wide16(c.v, es);
   a.wide_q = c.q.at && wide16(c.q, es) && wide16(c.qo, 2);
   a.table_rows = c.cos_t ? (int)c.table_rows : 0x7fffffff;
-  const long units = most_pages(c.n, c.s), qb = c.q.at ? (c.n + 3) / 4 : 0;
+  // query rows a wave: one until the waves fill the chip, then up to four (the search for a row's segment
+  // and its table rows are paid once a wave)
+  a.per = c.n >= 16384 ? 4 : c.n >= 8192 ? 2 : 1;
+  const long units = most_pages(c.n, c.s), qb = c.q.at ? (c.n + 4 * a.per - 1) / (4 * a.per) : 0;
   if (units * c.c.hkv + qb > 0x7fffffffL) return 2;
   a.units = (int)units;
   const dim3 grid((unsigned)(units * c.c.hkv + qb));
