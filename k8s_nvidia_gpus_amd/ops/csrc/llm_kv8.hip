@@ -1340,15 +1340,16 @@ long most_seen(const AttnCall& c, long rows) {
   return w < n ? w : n;
 }
 
-constexpr long kDecodeGrid = 768;                        // workgroups: three on each of the 256 CUs
+constexpr long kDecodeGrid = 512;                        // workgroups: two on each of the 256 CUs
 
 struct DecodePlan {
   int nw, per;
   long parts;
 };
-// Pages a wave: one until the workgroups fill the chip three deep, then as many as keep it so (a longer
-// chain of pages pays a workgroup's start and its partial output once).  Up to 8 pages run in one
-// workgroup of 8 waves, which needs no join.
+// Pages a wave: one until the workgroups fill the chip two deep, then as many as keep it so (a longer
+// chain of pages pays a workgroup's start and its partial output once): 8 x 32768 45 us, aiming at 768
+// workgroups 48, at 1024 51, at 384 50; 32 x 16000 with a window of 4000 61, 63, 67, 64.  Up to 8 pages
+// run in one workgroup of 8 waves, which needs no join: 500 positions 8.5 us against 11.
 DecodePlan decode_plan(const AttnCall& c) {
   const long n = most_seen(c, 1);
   if (n <= 8) return {8, 1, 1};
