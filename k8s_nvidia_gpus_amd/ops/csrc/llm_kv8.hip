@@ -168,6 +168,20 @@ __device__ __forceinline__ float block_scale(uint32_t bits) {
   return __uint_as_float((uint32_t)(max(e, -100) + 127) << 23);
 }
 
+// ---------------------------------------------------------------- across a wave
+// Inclusive scan of 64 lanes in six data-parallel-primitive steps (rows of 16, then across rows): a few
+// cycles each, where a shuffle takes an LDS round trip.  The last lane has the whole wave's.
+template <typename F>
+__device__ __forceinline__ int wave_scan(int x, int none, F f) {
+  x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x111, 0xf, 0xf, false));   // row_shr:1
+  x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x112, 0xf, 0xf, false));
+  x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x114, 0xf, 0xf, false));
+  x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x118, 0xf, 0xf, false));
+  x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x142, 0xa, 0xf, false));   // row_bcast:15
+  x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x143, 0xc, 0xf, false));   // row_bcast:31
+  return x;
+}
+
 // ---------------------------------------------------------------- ragged segments
 // Sequence s has rows cu[s] .. cu[s + 1] - 1 at positions start[s] ..; what is out of order, out of
 // [0, N) or at a negative start counts as empty.
@@ -199,12 +213,7 @@ __device__ __forceinline__ bool find_piece(const Segs& sg, int unit, F count, Pi
       sg.get(base + lane, row, n, pos);
       c = n > 0 ? count(n, pos) : 0;
     }
-    int inc = c;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(inc, o, 64);
-      if (lane >= o) inc += up;
-    }
+    const int inc = wave_scan(c, 0, [](int a, int b) { return a + b; });
     const uint64_t past = __ballot(before + inc > unit);
     if (past) {
       const int hit = __builtin_ctzll(past);
@@ -374,6 +383,17 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
   uint8_t* kc = a.c.k + sc * kPage * D;
   uint8_t* vc = a.c.v + sc * kPage * D;
   const float oldk = r0 ? a.c.ks[sc] : 0.f, oldv = r0 ? a.c.vs[sc] : 0.f;
+  // old value codes of 8 positions of 4 dims, where some of those are not new
+  constexpr int PV = D * 2 / 256 + (D * 2 % 256 != 0);
+  uint2 was[PV][4] = {};
+#pragma unroll
+  for (int u = 0; u < PV; ++u) {
+    const int i = tid + 256 * u, p0 = 8 * (i & 7), d = 4 * (i >> 3);
+    if (d < D && p0 < r1 && (p0 < r0 || p0 + 8 > r1)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) was[u][e] = *reinterpret_cast<const uint2*>(vc + (d + e) * kPage + p0);
+    }
+  }
   uint32_t mk = 0, mv = 0;                               // largest magnitudes, as bits (NaN largest)
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
@@ -384,12 +404,9 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
       mv = max(mv, max(__float_as_uint(vlo[u][e]) & 0x7fffffffu, __float_as_uint(vhi[u][e]) & 0x7fffffffu));
     }
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    mk = max(mk, (uint32_t)__shfl_xor((int)mk, o, 64));
-    mv = max(mv, (uint32_t)__shfl_xor((int)mv, o, 64));
-  }
-  if (lane == 0) { red[0][wave] = mk; red[1][wave] = mv; }
+  mk = wave_scan(mk, 0, [](int a, int b) { return max(a, b); });   // (31 bits: they order as integers do)
+  mv = wave_scan(mv, 0, [](int a, int b) { return max(a, b); });
+  if (lane == 63) { red[0][wave] = mk; red[1][wave] = mv; }
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 4; ++w) { mk = max(mk, red[0][w]); mv = max(mv, red[1][w]); }
@@ -433,7 +450,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
   // 8 positions of 4 dims a thread: eight lanes write a dim's 64 bytes
   const float rv = growv ? oldv * iv : 1.f;
 #pragma unroll
-  for (int u = 0; u < D * 2 / 256 + (D * 2 % 256 != 0); ++u) {
+  for (int u = 0; u < PV; ++u) {
     const int i = tid + 256 * u, p0 = 8 * (i & 7), d = 4 * (i >> 3);
     const bool has_new = p0 < r1 && p0 + 8 > r0;
     if (d >= D || (!has_new && !(growv && p0 < r0))) continue;
@@ -454,7 +471,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
       uint2* at = reinterpret_cast<uint2*>(vc + (d + e) * kPage + p0);
       uint2 w = make_uint2(lo[e], hi[e]);
       if (keep[0] | keep[1]) {
-        uint2 old = *at;
+        uint2 old = was[u][e];
         if (growv) { old.x = rescale4<FP8>(old.x, rv); old.y = rescale4<FP8>(old.y, rv); }
         w.x = (w.x & ~keep[0]) | (old.x & keep[0]);
         w.y = (w.y & ~keep[1]) | (old.y & keep[1]);
@@ -620,11 +637,35 @@ struct AttnArgs {
   float* dx;
   float* sx;
   long sq_tok, sq_head, so_tok, so_head;
-  int H, G, span, window, sinks, parts, units;
+  int H, G, D, span, window, sinks, parts, units;
   int per;                 // decode: pages a wave (at most 64)
   float c2, sign;          // |scale| x log2(e), and its sign (goes into the query)
   bool wide_q, wide_o;
 };
+
+// N consecutive output values at column `col` of row t as Q8: int8 with a scale for each 32 columns and
+// the scaled sum of each 16 (neighbouring lanes hold neighbouring columns; blocks begin at lane groups).
+template <int N>
+__device__ __forceinline__ void put_q8(const AttnArgs& a, int t, long col, const float (&y)[N]) {
+  const long at = (long)t * a.H * a.D + col;
+  float amax = fabsf(y[0]);
+#pragma unroll
+  for (int e = 1; e < N; ++e) amax = fmaxf(amax, fabsf(y[e]));
+#pragma unroll
+  for (int o = 16 / N; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+  const float d = amax / 127.f;
+  int sum = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const int c = d > 0.f ? (int)__builtin_rintf(y[e] / d) : 0;
+    a.x8[at + e] = (int8_t)c;
+    sum += c;
+  }
+#pragma unroll
+  for (int o = 8 / N; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if ((col & 31) == 0) a.dx[at >> 5] = d;
+  if ((col & 15) == 0) a.sx[at >> 4] = d * (float)sum;
+}
 
 // Single-token attention.  Grid (Hkv x groups of 16 heads, parts, S); workgroup part p streams pages
 // p NW per .. of the row's list, each wave whole pages with its own online softmax, no LDS and no barrier
@@ -744,11 +785,12 @@ __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a
     const bool whole = base + kPage - 1 <= last &&
                        (a.window <= 0 || base > pos - a.window || base + kPage <= a.sinks);
     if (!whole) {                                        // a border inside the page (wave-uniform)
+      const int at = base + 16 * kg, hi = last - at;     // of the registers' own offsets
+      const int lo = (a.window > 0 ? pos - a.window : -1) - at, sinks = a.sinks - at;
       uint32_t keep[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int j = base + 16 * kg + e;
-        const bool in = j <= last && (a.window <= 0 || j > pos - a.window || j < a.sinks);
+        const bool in = (e <= hi) & ((e > lo) | (e < sinks));
         sc[e] = in ? sc[e] : -INFINITY;
         keep[e >> 2] |= in ? 0xffu << (8 * (e & 3)) : 0u;
       }
@@ -828,15 +870,17 @@ __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a
       if (e != 0.f) y += *reinterpret_cast<f4*>(&wo[w][g][d]) * e;
     }
     const int h = kh * a.G + h0 + g;
-    if (a.parts > 1 || a.x8) {
+    if (a.parts > 1) {
       const long row = ((long)part * a.sg.N + t) * a.H + h;
       *reinterpret_cast<f4*>(a.po + row * D + d) = y;
       if (d == 0) { a.pml[2 * row] = M; a.pml[2 * row + 1] = L; }
     } else {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
+      y *= L == 0.f ? 0.f : 1.f / L;
+      if (a.x8) put_q8<4>(a, t, (long)h * D + d, {y[0], y[1], y[2], y[3]});
+      if (!a.out) continue;
       uint16_t* at = static_cast<uint16_t*>(a.out) + (long)t * a.so_tok + (long)h * a.so_head + d;
-      const uint32_t w0 = Elem<T>::put(y[0] * inv) | (uint32_t)Elem<T>::put(y[1] * inv) << 16;
-      const uint32_t w1 = Elem<T>::put(y[2] * inv) | (uint32_t)Elem<T>::put(y[3] * inv) << 16;
+      const uint32_t w0 = Elem<T>::put(y[0]) | (uint32_t)Elem<T>::put(y[1]) << 16;
+      const uint32_t w1 = Elem<T>::put(y[2]) | (uint32_t)Elem<T>::put(y[3]) << 16;
       if (a.wide_o) {
         *reinterpret_cast<uint2*>(at) = make_uint2(w0, w1);
       } else {
@@ -921,24 +965,8 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) at[e] = Elem<T>::put(y[e]);
   }
-  if (DECODE && a.x8) {                                  // Q8: blocks of 32 dims, sums of 16
-    const long K = (long)a.H * D, col = (long)h * D + E * lane;
-    float amax = fabsf(y[0]);
-    if (E > 1) amax = fmaxf(amax, fabsf(y[E - 1]));
-#pragma unroll
-    for (int o = 16 / E; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-    const float d = amax / 127.f;
-    int sum = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = d > 0.f ? (int)__builtin_rintf(y[e] / d) : 0;
-      a.x8[t * K + col + e] = (int8_t)c;
-      sum += c;
-    }
-#pragma unroll
-    for (int o = 8 / E; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if ((col & 31) == 0) a.dx[(t * K + col) >> 5] = d;
-    if ((col & 15) == 0) a.sx[(t * K + col) >> 4] = d * (float)sum;
+  if constexpr (DECODE) {
+    if (a.x8) put_q8<E>(a, t, (long)h * D + E * lane, y);
   }
 }
 
@@ -1323,7 +1351,7 @@ AttnArgs make_attn(const AttnCall& c, float scale, void* work, long parts) {
   a.dx = ptr<float>(c.dx);
   a.sx = ptr<float>(c.sx);
   a.sq_tok = c.q.tok; a.sq_head = c.q.head; a.so_tok = c.out.tok; a.so_head = c.out.head;
-  a.H = (int)c.heads; a.G = (int)(c.heads / c.c.hkv);
+  a.H = (int)c.heads; a.G = (int)(c.heads / c.c.hkv); a.D = (int)c.c.d;
   a.span = (int)c.span; a.window = (int)c.window; a.sinks = (int)c.sinks; a.parts = (int)parts;
   a.c2 = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
   a.sign = scale < 0.f ? -1.f : 1.f;
@@ -1474,7 +1502,7 @@ long amdk8s_llm_kv8_decode_work(const void* call) {
   const AttnCall& c = *static_cast<const AttnCall*>(call);
   if (!good_attn(c) || !in(c.s, 1, 65535) || c.n != c.s) return -1;
   const long parts = decode_plan(c).parts;
-  return parts == 1 && !c.x8 ? 0 : parts * c.n * c.heads * (c.c.d + 2);
+  return parts == 1 ? 0 : parts * c.n * c.heads * (c.c.d + 2);
 }
 
 // One query row a sequence at position start[s] (-1: nothing to see, zeros); keys at or behind `span` are
