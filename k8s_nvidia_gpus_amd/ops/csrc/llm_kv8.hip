@@ -191,7 +191,7 @@ struct Segs {
   int S, N;
   __device__ __forceinline__ void get(int s, int& row, int& n, int& pos) const {
     row = max(cu[s], 0);
-    n = min(cu[s + 1], N) - row;
+    n = max(min(cu[s + 1], N), 0) - row;
     pos = start[s];
     if (pos < 0 || pos > 0x3fffffff) n = 0;
   }
@@ -249,7 +249,7 @@ __device__ __forceinline__ bool find_row(const Segs& sg, int n, Row& out) {
 
 __device__ __forceinline__ int pages_of(int n, int pos) { return (pos + n - 1) / kPage - pos / kPage + 1; }
 
-// most pieces of `each` rows (pages: of any alignment) that N rows in S segments make
+// most pages that N rows in S segments touch, whatever their positions
 inline long most_pages(long N, long S) {
   const long m = (N + 62 * S) / 64 + S;
   return m < N ? m : N;
@@ -315,9 +315,13 @@ __device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const float
 // Blocks [0, units * Hkv): one page of one sequence and KV head each, 256 threads: the new rows' keys
 // are rotated, the page's new scale is the larger of the old one (if the page was begun before) and
 // the new rows' own, old codes are shifted if it grew, the new rows' codes are written.  One block owns
-// the page's codes and scales, so there are no atomics.  The blocks behind rotate the queries, a wave a
-// row.  Memory-bound: 16-byte loads and stores of whole rows; a value code row of 64 positions is
-// written in 16-byte pieces through an LDS transpose.
+// the page's codes and scales, so there are no atomics.  The blocks behind rotate the queries, `per` rows
+// a wave, a lane's pairs the same in every head (its table entries are read once a row).  Memory-bound:
+// 16-byte loads and stores of whole rows; values change their order on the way, through LDS and 4 x 4
+// byte transposes in registers, eight lanes writing a dim's 64 positions.  12800 tokens of 28 + 4 + 4
+// heads behind 8 x 1500: 55 us, 4.0 TB/s (14 us without the queries); a token for each of 4 sequences
+// 5.5 us, of it about 2 us the launch: segment search, page entry and scale, the block's maximum and the
+// stores wait for each other.
 template <int D, bool FP8, int T, int TO>
 __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
   typedef typename Elem<T>::type E;
@@ -491,7 +495,8 @@ struct ReadArgs {
   bool wide;
 };
 
-// one page of one sequence and KV head a block: keys row by row, values through an LDS transpose
+// One page of one sequence and KV head a block: keys row by row, values through byte transposes and LDS.
+// Memory-bound, two thirds of it the values' stores: 8 x 16384 positions 68 us, 4.3 TB/s.
 template <int D, bool FP8, int T>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
   typedef typename Elem<T>::type E;
@@ -648,12 +653,12 @@ struct AttnArgs {
 template <int N>
 __device__ __forceinline__ void put_q8(const AttnArgs& a, int t, long col, const float (&y)[N]) {
   const long at = (long)t * a.H * a.D + col;
-  float amax = fabsf(y[0]);
+  uint32_t top = 0;                                      // as bits: a NaN makes its block's scale NaN
 #pragma unroll
-  for (int e = 1; e < N; ++e) amax = fmaxf(amax, fabsf(y[e]));
+  for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
 #pragma unroll
-  for (int o = 16 / N; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-  const float d = amax / 127.f;
+  for (int o = 16 / N; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+  const float d = __uint_as_float(top) / 127.f;
   int sum = 0;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
@@ -676,7 +681,10 @@ __device__ __forceinline__ void put_q8(const AttnArgs& a, int t, long col, const
 //   dim: the same positions as its scores, so neither P nor V moves between lanes.  The running
 //   maximum, sum and rescaling are one head's, a lane's own.
 // A page's keys are loaded as soon as the last page's have been used, and its values likewise: 16 KB in
-// flight a wave most of the time at half the registers of two buffers.
+// flight a wave most of the time at half the registers of two buffers, so three waves fit a SIMD (two
+// buffers left one; 32 x 16000 with a window 140 us, this 61).  Bound by the cache's bytes: 8 x 32768
+// in e4m3 45 us, 4.7 TB/s, where a copy reaches 5.1; short contexts by launches (two, 2 to 3 us each) and
+// the chain position, page entry, page, join: 8 x 4096 13.4 us, 500 positions 8.1.
 template <int D, bool FP8, int T, int NW>
 __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a) {
   constexpr int KH = D / 64, ND = D / 16;
@@ -695,6 +703,14 @@ __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a
   const Seen seen = seen_pages(pos, pos, a.span, a.window, a.sinks);
   const int mine = max(0, min(a.per, (seen.n - p0 - wave + NW - 1) / NW));
   if (a.window > 0 && lane < mine) my_id = a.c.page(t, seen.page(p0 + wave + NW * lane));
+  if (part > 0 && p0 >= seen.n) {                        // nothing of the row here: an empty partial
+    if ((int)threadIdx.x < gn) {
+      float* ml = a.pml + 2 * (((long)part * a.sg.N + t) * a.H + kh * a.G + h0 + threadIdx.x);
+      ml[0] = -INFINITY;
+      ml[1] = 0.f;
+    }
+    return;
+  }
   float my_ks = 0.f, my_vs = 0.f;
   if (lane < mine && my_id >= 0) {
     const long sc = (long)my_id * a.c.Hkv + kh;
@@ -977,6 +993,12 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
 // v_mfma_f32_32x32x16_f16, a lane owns one query row: softmax and rescaling need one exchange (lane
 // ^ 32).  The key of position p lies in LDS row p with bits 2 and 3 swapped, so that the score
 // registers of a lane are, in order, the P operand's consecutive positions: P never moves.
+// What bounds it: matrix and vector instructions of a SIMD's two waves hardly overlap (8192 rows at 0:
+// matrix cores busy 48 % of the time, vector units 50 %), and half of the vector time is the exponents.
+// 8192 at 0 500 us, 960 TFLOP/s of visible pairs (a library product of two 8192 matrices reaches 1450);
+// 512 at 31488 250 us.  Tried and not taken: 64 rows a wave (twice the registers, one wave a SIMD: 660
+// us), the next page's scores ahead of this page's weights (580), pages turned to fp16 images in memory
+// once and loaded into LDS directly (503, and 284 for 512 at 31488), wave priorities (no change).
 __device__ __forceinline__ int swap23(int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); }
 
 // A tile's LDS image: key rows of 2 D bytes and value rows of 128 (64 positions of a dim) in fp16, each
@@ -1410,7 +1432,7 @@ PromptPlan prompt_plan(const AttnCall& c) {
     const long own = c.n / (kPage * c.s);
     const double mean = n - 0.5 * (own < n ? own : n);
     const double bytes = 8.0 * c.n * c.heads * c.c.d;
-    for (long p = 1; p <= n && p <= 64; ++p) {
+    for (long p = 1; p <= n && p <= (c.n > 65535 ? 1 : 64); ++p) {   // (the join's grid has 16 bits of rows)
       const long wgs = units * c.c.hkv * p;
       const double crowd = (wgs * mean / n - 256) / 128;  // CUs with two workgroups: none to most
       const double page = nw == 8 ? 1.95 : 1.5 + 0.55 * (crowd < 0 ? 0 : crowd > 1 ? 1 : crowd);

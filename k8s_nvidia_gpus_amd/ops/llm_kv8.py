@@ -165,8 +165,9 @@ def kv8_append(cache: Sequence[torch.Tensor], k: torch.Tensor, v: torch.Tensor, 
 
     A page that is begun (its first position is among the rows) takes the rows' own scale; one that was
     begun before keeps the larger scale, its earlier codes shifted to it.  What lies behind the last
-    appended position of a page is dead.  A page must be appended to by one sequence of a call only
-    (shared prefix pages are for reading)."""
+    appended position of a page is dead.  What lies behind the table is dropped.  A page must be appended
+    to by one sequence of a call only (shared prefix pages are for reading), and a page that is entered
+    behind its first position must have scales (zeros, if nothing was written: :meth:`KV8Cache.empty`)."""
     what = "kv8_append"
     dev, hkv, d, s, columns, pool = _pool(what, cache, pages)
     kind = k.dtype

@@ -330,6 +330,16 @@ def test_decode_q8_of_a_short_context(KV, d):
         check(out[s:s + 1], reference(cache, rows[s], q[s:s + 1], n - 1, 1 / math.sqrt(d)))
 
 
+@pytest.mark.parametrize("n", [300, 3000])
+def test_decode_q8_of_a_poisoned_page_is_not_silent(KV, n):
+    cache, rows, q, pos = decode_case(KV, [n, n], 8, 2, 128, "int8", torch.float16, seed=17)
+    cache.vs[rows[0][1], 1] = float("nan")
+    x8 = torch.empty(2, 1024, dtype=torch.int8, device=DEV)
+    dx, sx = torch.empty(2, 32, device=DEV), torch.empty(2, 64, device=DEV)
+    KV.kv8_attn_decode(q, cache, ints(rows), pos, None, 1 / math.sqrt(128), q8_out=(x8, dx, sx))
+    assert dx[0, 16:].isnan().all() and dx[0, :16].isfinite().all() and dx[1].isfinite().all()
+
+
 def test_decode_offsets_pass_32_bits(KV):
     pool, hkv, d = 33100, 8, 128                            # 2.17 GB of key codes, as many of values
     cache = KV.KV8Cache.empty(pool, hkv, d, torch.int8, DEV)
@@ -398,6 +408,14 @@ def test_prompt_long(KV, starts, lens, h, hkv):
     check_prompt(cache, rows, q, starts, lens, run_prompt(KV, cache, rows, q, starts, lens))
 
 
+def test_prompt_of_more_rows_than_a_join_takes(KV):
+    n, at = 66000, [0, 1, 4000, 65535, 65536, 65999]
+    cache, rows, q = prompt_case(KV, [0], [n], 1, 1, 64, "int8", torch.float16, seed=9)
+    got = run_prompt(KV, cache, rows, q, [0], [n])
+    for i in at:
+        check(got[i:i + 1], reference(cache, rows[0], q[i:i + 1], i, 1 / 8))
+
+
 @pytest.mark.parametrize("window,sinks", WINDOWS)
 @pytest.mark.parametrize("code", CODES)
 def test_prompt_window_and_sinks(KV, code, window, sinks):
@@ -444,6 +462,26 @@ def test_prompt_a_poisoned_page_reaches_only_rows_that_see_it(KV):
     cache.vs[rows[0][2], 0] = float("nan")                   # positions 128..191
     got = run_prompt(KV, cache, rows, q, starts, lens)
     assert got[:128].isfinite().all() and got[128:, :4].isnan().all() and got[:, 4:].isfinite().all()
+
+
+@pytest.mark.parametrize("cu", [[0, -2 ** 31, 70, 100], [2 ** 31 - 1, 0, 50, 100], [90, 20, 60, 2 ** 31 - 1]])
+def test_segments_out_of_order(KV, cu):
+    """Nothing out of range is touched, and what is in a segment that makes sense is right."""
+    g = torch.Generator(device=DEV).manual_seed(19)
+    cache, rows, q = prompt_case(KV, [0, 0, 0], [100, 100, 100], 8, 2, 64, "int8", torch.float16, seed=19)
+    q, out = q[:100], torch.full_like(q[:100], 7.0)
+    x = torch.randn(100, 2, 64, device=DEV, generator=g)
+    k, v = torch.full_like(x, 7.0), torch.full_like(x, 7.0)
+    KV.kv8_attn_prompt(q, cache, ints(rows), ints([0, 0, 0]), ints(cu), out, 1 / 8)
+    KV.kv8_read(cache, ints(rows), ints([0, 0, 0]), ints(cu), k, v)
+    for s in range(3):
+        a, b = max(cu[s], 0), min(cu[s + 1], 100)
+        if a < b and sorted(cu)[2:] == cu[2:] and s == 2:
+            check(out[a:b], reference(cache, rows[s], q[a:b], 0, 1 / 8))
+    before = clone(KV, cache)
+    KV.kv8_append(cache, x, x, ints(rows), ints([0, 0, 0]), ints(cu), q=q.float(), q_out=out)
+    spare = [i for i in range(cache.k.shape[0]) if i not in {i for r in rows for i in r}]
+    assert torch.equal(bits(cache.k)[spare], bits(before.k)[spare])
 
 
 def test_prompt_bad_segments_are_left_alone(KV):
