@@ -182,6 +182,19 @@ __device__ __forceinline__ int wave_scan(int x, int none, F f) {
   return x;
 }
 
+__device__ __forceinline__ float wave_max(float x) {
+  const int r = wave_scan(__float_as_int(x), (int)0xff800000, [](int a, int b) {
+    return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b)));
+  });
+  return __int_as_float(__builtin_amdgcn_readlane(r, 63));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  const int r = wave_scan(__float_as_int(x), 0, [](int a, int b) {
+    return __float_as_int(__int_as_float(a) + __int_as_float(b));
+  });
+  return __int_as_float(__builtin_amdgcn_readlane(r, 63));
+}
+
 // ---------------------------------------------------------------- ragged segments
 // Sequence s has rows cu[s] .. cu[s + 1] - 1 at positions start[s] ..; what is out of order, out of
 // [0, N) or at a negative start counts as empty.
@@ -938,16 +951,10 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
     float pm = a.pml[2 * at], pl = a.pml[2 * at + 1];
     load(wave);
     if (lane >= n) { pm = -INFINITY; pl = 0.f; }
-    float mx = pm;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    const float mn = fmaxf(M, mx);
+    const float mn = fmaxf(M, wave_max(pm));
     const float al = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn);
     const float w = pm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(pm - mn);
-    float ls = pl != pl ? pl : pl * w;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o, 64);
-    L = L * al + ls;
+    L = L * al + wave_sum(pl != pl ? pl : pl * w);
     M = mn;
 #pragma unroll
     for (int e = 0; e < E; ++e) y[e] *= al;
@@ -994,7 +1001,8 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
 // ^ 32).  The key of position p lies in LDS row p with bits 2 and 3 swapped, so that the score
 // registers of a lane are, in order, the P operand's consecutive positions: P never moves.
 // What bounds it: matrix and vector instructions of a SIMD's two waves hardly overlap (8192 rows at 0:
-// matrix cores busy 48 % of the time, vector units 50 %), and half of the vector time is the exponents.
+// matrix cores busy 42 % of the time, vector units 48 %), and half of the vector time is the exponents;
+// three waves a SIMD took 12 % fewer cycles at a clock 11 % lower.
 // 8192 at 0 500 us, 960 TFLOP/s of visible pairs (a library product of two 8192 matrices reaches 1450);
 // 512 at 31488 250 us.  Tried and not taken: 64 rows a wave (twice the registers, one wave a SIMD: 660
 // us), the next page's scores ahead of this page's weights (580), pages turned to fp16 images in memory
