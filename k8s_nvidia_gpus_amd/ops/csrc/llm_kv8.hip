@@ -1404,16 +1404,23 @@ struct DecodePlan {
   int nw, per;
   long parts;
 };
-// Pages a wave: one until the workgroups fill the chip two deep, then as many as keep it so (a longer
-// chain of pages pays a workgroup's start and its partial output once): 8 x 32768 45 us, aiming at 768
-// workgroups 48, at 1024 51, at 384 50; 32 x 16000 with a window of 4000 61, 63, 67, 64.  Up to 8 pages
-// run in one workgroup of 8 waves, which needs no join: 500 positions 8.5 us against 11.
+// Workgroups that share a row's pages: as many as let 512 workgroups, two on each CU, take all rows in one
+// round (8 x 32768 44 us; at most 384 49; 576 and more, a second round, 48; 32 x 16000 in 4 parts 98, in
+// 5 112).  At most 64, past which the join costs what the shorter chains save (1 x 32768 in 64 parts 13.9,
+// in 128 16.0), unless a wave would have more than the 64 pages whose table entries it holds.  Where one
+// part fills the CUs, a wave has 4 pages before there is a second one (64 x 1000 in one part 14.7, in two
+// 18.5); where it does not, one page is enough (1 x 4000 with one page a wave 9.1, with two 10.7).  Up to
+// 8 pages run in one workgroup of 8 waves, which needs no join: 500 positions 8.1 us against 9.2.
 DecodePlan decode_plan(const AttnCall& c) {
   const long n = most_seen(c, 1);
   if (n <= 8) return {8, 1, 1};
   const long chains = c.s * c.c.hkv * ((c.heads / c.c.hkv + 15) / 16);
-  long per = chains * n / (4 * kDecodeGrid);
-  per = per < 1 ? 1 : per > 64 ? 64 : per;
+  const long fill = kDecodeGrid / chains, few = chains >= kDecodeGrid / 2 ? 4 : 1;
+  const long worth = (n + 4 * few - 1) / (4 * few), need = (n + 255) / 256;
+  long parts = fill > 64 ? 64 : fill;
+  parts = parts > worth ? worth : parts;
+  parts = parts < need ? need : parts;
+  const long per = (n + 4 * parts - 1) / (4 * parts);
   return {4, (int)per, (n + 4 * per - 1) / (4 * per)};
 }
 
