@@ -242,7 +242,8 @@ __device__ __forceinline__ bool find_piece(const Segs& sg, int unit, F count, Pi
   return false;
 }
 
-// The segment that row n is in (the whole wave asks for one row): its rows row .. end - 1, at pos ...
+// The segment that row n is in (the whole wave asks for one row): its rows row .. end - 1, at pos ...  False,
+// and end = 0: none.
 struct Row {
   int row, end, pos;
 };
@@ -256,8 +257,9 @@ __device__ __forceinline__ bool find_row(const Segs& sg, int n, Row& out) {
   if (s >= sg.S) return false;
   int cnt;
   sg.get(s, out.row, cnt, out.pos);
-  out.end = out.row + cnt;
-  return n >= out.row && n < out.end;
+  const bool in = n >= out.row && n < out.row + cnt;
+  out.end = in ? out.row + cnt : 0;
+  return in;
 }
 
 __device__ __forceinline__ int pages_of(int n, int pos) { return (pos + n - 1) / kPage - pos / kPage + 1; }

@@ -168,6 +168,42 @@ def test_decode_long(KV, n):
         check(got[s:s + 1], reference(cache, rows[s], q[s:s + 1], m - 1, 1 / math.sqrt(128)))
 
 
+@pytest.mark.parametrize("s,pages", [(1, 65), (3, 9), (64, 9), (64, 17), (64, 33), (129, 10), (70, 130)])
+def test_decode_many_rows_share_pages(KV, s, pages):
+    """Parts by the number of rows; the rows' tables name the same pages in other orders."""
+    g = torch.Generator(device=DEV).manual_seed(60)
+    cache = random_cache(KV, 40, 4, 128, "e4m3", g)
+    table = torch.randint(0, 40, (s, pages), device=DEV, generator=g, dtype=torch.int32)
+    pos = torch.randint(0, pages * PAGE, (s,), device=DEV, generator=g, dtype=torch.int32)
+    pos[-1] = pages * PAGE - 1
+    q = torch.randn(s, 8, 128, device=DEV, generator=g).half()
+    out = torch.full_like(q, float("nan"))
+    KV.kv8_attn_decode(q, cache, table, pos, out, 0.08)
+    rows, at = table.tolist(), pos.tolist()
+    for i in {0, s // 2, s - 1}:
+        check(out[i:i + 1], reference(cache, rows[i], q[i:i + 1], at[i], 0.08))
+
+
+def test_decode_more_than_a_million_positions(KV):
+    """More pages than 64 parts of four waves hold table entries for; few distinct ones, so that the plain
+    form is a sum over those: page u is seen n_u times and the last one up to the position."""
+    g = torch.Generator(device=DEV).manual_seed(61)
+    cache = random_cache(KV, 8, 1, 64, "int8", g, spread=0.01)
+    pages, scale = 16500, 0.1
+    table = torch.randint(0, 7, (1, pages), device=DEV, generator=g, dtype=torch.int32)
+    table[0, -1] = 7                                        # the last page is its own
+    pos = pages * PAGE - 10
+    q = torch.randn(1, 4, 64, device=DEV, generator=g).half()
+    out = torch.empty_like(q)
+    KV.kv8_attn_decode(q, cache, table, ints([pos]), out, scale)
+    count = torch.bincount(table[0].long(), minlength=8).double().repeat_interleave(PAGE)
+    count[-9:] = 0
+    k, v, _ = dense(cache, list(range(8)), 0, 8 * PAGE)
+    w = torch.exp((q[0].double() @ k.t()) * scale) * count
+    w /= w.sum(-1, keepdim=True)
+    check(out, ((w @ v)[None], (w @ v.abs())[None], pages * PAGE, float(v.abs().max())))
+
+
 WINDOWS = [(1, 0), (1, 1), (64, 0), (65, 4), (100, 64), (130, 70), (5000, 3), (7, 1000)]
 
 
@@ -701,6 +737,23 @@ def test_append_strides_and_in_place_rotation(KV):
 
 
 # -------------------------------------------------------------------------------------------------- read
+@pytest.mark.parametrize("first", [0, 1, 6, 4099])
+def test_append_rows_before_the_first_sequence_are_left_alone(KV, first):
+    n, rest, d = 8300, 37, 64                               # enough rows that a wave takes several
+    cos, sin = tables(200 * PAGE, d)
+    cache = KV.KV8Cache.empty(140, 1, d, torch.int8, DEV)
+    g = torch.Generator(device=DEV).manual_seed(50)
+    x = torch.randn(n, 4, d, device=DEV, generator=g).half()
+    table, out = ints([list(range(135))]), torch.full((n, 2, d), 7.0, device=DEV, dtype=torch.float16)
+    KV.kv8_append(cache, x[:, 2:3], x[:, 3:], table, ints([2]), ints([first, n - rest]), cos, sin, q=x[:, :2], q_out=out)
+    want, ref = KV.KV8Cache.empty(140, 1, d, torch.int8, DEV), torch.empty_like(out)
+    y = x[first:n - rest]
+    KV.kv8_append(want, y[:, 2:3], y[:, 3:], table, ints([2]), ints([0, len(y)]), cos, sin, q=y[:, :2], q_out=ref[:len(y)])
+    assert torch.equal(out[first:n - rest], ref[:len(y)])
+    assert (out[:first] == 7.0).all() and (out[n - rest:] == 7.0).all()
+    assert all(torch.equal(a, b) for a, b in zip(cache, want))
+
+
 @pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("d", [64, 128])
