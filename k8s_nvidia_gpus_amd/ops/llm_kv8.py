@@ -137,6 +137,16 @@ def _rows(what: str, name: str, t: torch.Tensor, n: int, heads: int, d: int, dev
     return t.data_ptr(), strides[0], strides[1]
 
 
+def _out_rows(what: str, name: str, t: torch.Tensor, n: int, heads: int, d: int, dev: int) -> Tuple[int, int, int]:
+    """`_rows` of an output: its rows must not share memory (an expanded view would)."""
+    rows = _rows(what, name, t, n, heads, d, dev)
+    _, row, head = rows
+    if (heads > 1 and head < d) or (n > 1 and row < d) \
+            or (n > 1 and heads > 1 and row < (heads - 1) * head + d and head < (n - 1) * row + d):
+        _bad(what, f"{name} {tuple(t.shape)} / {t.stride()}: its rows overlap")
+    return rows
+
+
 def _gpu(what: str, dev: int) -> None:
     if dev < 0:
         _bad(what, "the tensors are not on a GPU, and the kernels run nowhere else")
@@ -173,7 +183,7 @@ def kv8_append(cache: Sequence[torch.Tensor], k: torch.Tensor, v: torch.Tensor, 
     kind = k.dtype
     if kind not in _TYPES or v.dtype != kind:
         _bad(what, f"k is {kind}, v {v.dtype}: one type of fp16, bf16, fp32")
-    n = k.shape[0]
+    n = k.shape[0] if k.dim() == 3 else -1
     kp, vp = _rows(what, "k", k, n, hkv, d, dev), _rows(what, "v", v, n, hkv, d, dev)
     starts, cus = _ints(what, "start", start, s, dev), _ints(what, "cu", cu, s + 1, dev)
     if (cos_t is None) != (sin_t is None) or (q is None) != (q_out is None):
@@ -192,11 +202,11 @@ def kv8_append(cache: Sequence[torch.Tensor], k: torch.Tensor, v: torch.Tensor, 
     qp = op = _NONE
     heads, otype = 0, kind
     if q is not None:
-        heads, otype = q.shape[1], q_out.dtype
+        heads, otype = q.shape[1] if q.dim() == 3 and q.shape[1] else -1, q_out.dtype
         if q.dtype != kind or otype not in _QTYPES or (kind != _F32 and otype != kind):
             _bad(what, f"q is {q.dtype}, q_out {otype}: q of k's type ({kind}), q_out the same, or fp16 or "
                        f"bf16 for fp32")
-        qp, op = _rows(what, "q", q, n, heads, d, dev), _rows(what, "q_out", q_out, n, heads, d, dev)
+        qp, op = _rows(what, "q", q, n, heads, d, dev), _out_rows(what, "q_out", q_out, n, heads, d, dev)
     _gpu(what, dev)
     if n:
         _launch(what, dev, _lib().amdk8s_llm_kv8_append,
@@ -211,10 +221,10 @@ def kv8_read(cache: Sequence[torch.Tensor], pages: torch.Tensor, start: torch.Te
     unmapped pages read as zeros."""
     what = "kv8_read"
     dev, hkv, d, s, _, pool = _pool(what, cache, pages)
-    kind, n = k_out.dtype, k_out.shape[0]
+    kind, n = k_out.dtype, k_out.shape[0] if k_out.dim() == 3 else -1
     if kind not in _TYPES or v_out.dtype != kind:
         _bad(what, f"k_out is {kind}, v_out {v_out.dtype}: one type of fp16, bf16, fp32")
-    kp, vp = _rows(what, "k_out", k_out, n, hkv, d, dev), _rows(what, "v_out", v_out, n, hkv, d, dev)
+    kp, vp = _out_rows(what, "k_out", k_out, n, hkv, d, dev), _out_rows(what, "v_out", v_out, n, hkv, d, dev)
     starts, cus = _ints(what, "start", start, s, dev), _ints(what, "cu", cu, s + 1, dev)
     _gpu(what, dev)
     if n:
@@ -234,7 +244,7 @@ def _attention(what, q, out, hkv, d, dev, columns, span, window, sinks):
     if out is not None:
         if out.dtype != kind:
             _bad(what, f"out is {out.dtype}, q {kind}")
-        op = _rows(what, "out", out, n, heads, d, dev)
+        op = _out_rows(what, "out", out, n, heads, d, dev)
     most = columns * PAGE
     span = span or most
     if not 0 < span <= most:

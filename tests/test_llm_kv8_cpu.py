@@ -38,6 +38,17 @@ def test_a_right_call_gets_as_far_as_the_device(name):
         CALLS[name](**good(name))
 
 
+@pytest.mark.parametrize("layout", [
+    lambda z: z(H, N, D).transpose(0, 1),                    # head-major
+    lambda z: z(N, H + 3, 2 * D)[:, 1:-2, D:],
+    lambda z: z(H, 2 * N, D)[:, ::2].transpose(0, 1),
+])
+def test_outputs_of_any_layout_whose_rows_are_their_own_are_taken(layout):
+    out = layout(lambda *shape: torch.zeros(shape, dtype=torch.float16))
+    with pytest.raises(ValueError, match="GPU"):
+        KV.kv8_attn_prompt(**{**good("prompt"), "out": out})
+
+
 def with_cache(i, t):
     def change(a):
         c = list(a["cache"])
@@ -83,11 +94,19 @@ OWN = {
         (with_arg("q_out", lambda t: t.float()), "q_out"),
         (with_arg("q", lambda t: t.float()), "type"),
         (with_arg("q", lambda t: t[:-1]), "q "),
+        (with_arg("q", lambda t: t[0]), "q "),
+        (with_arg("q", lambda t: t[:, :0]), "q "),
+        (with_arg("k", lambda t: t[0, 0]), "k "),
+        (with_arg("q_out", lambda t: t[:1].expand(N, H, D)), "overlap"),
+        (with_arg("q_out", lambda t: t.view(-1).as_strided((N, H, D), (H * D // 2, D // 2, 1))), "overlap"),
     ],
     "read": [
         (with_arg("k_out", lambda t: t.double()), "type"),
         (with_arg("v_out", lambda t: t[:-1]), "v_out"),
         (with_arg("cu", lambda t: t.float()), "cu"),
+        (with_arg("k_out", lambda t: t[0, 0, 0]), "k_out"),
+        (with_arg("k_out", lambda t: t[:, :1].expand(N, HKV, D)), "overlap"),
+        (with_arg("v_out", lambda t: t[:1].expand(N, HKV, D)), "overlap"),
     ],
     "decode": [
         (with_arg("q", lambda t: t[:, :3]), "multiple"),
@@ -95,6 +114,7 @@ OWN = {
         (with_arg("q", lambda t: t[:1]), "out"),
         (with_arg("out", lambda t: t.bfloat16()), "out"),
         (with_arg("out", None), "neither"),
+        (with_arg("out", lambda t: t[:1].expand(S, H, D)), "overlap"),
         (with_arg("pos", lambda t: t[:1]), "pos"),
         (with_arg("window", -1), "window"),
         (with_arg("sinks", 1 << 31), "sinks"),
@@ -110,6 +130,7 @@ OWN = {
         (with_arg("start", lambda t: t[:1]), "start"),
         (with_arg("cu", lambda t: t[:2]), "cu"),
         (with_arg("out", None), "out"),
+        (with_arg("out", lambda t: t.view(-1).as_strided((N, H, D), (D, D, 1))), "overlap"),
         (with_arg("span", 1000), "span"),
     ],
 }
