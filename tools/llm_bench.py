@@ -190,8 +190,12 @@ def main(argv=None) -> int:
                     default=int(os.environ.get("AMDK8S_LLM_NORM_PROLOGUE_T", "0")),
                     help="A/B: steps of up to this many tokens normalise in the GEMV prologues "
                          "(0 = the engine default; env AMDK8S_LLM_NORM_PROLOGUE_T)")
+    ap.add_argument("--cache-type", choices=["f16", "int8", "e4m3"], default="f16",
+                    help="KV cache elements")
     ap.add_argument("--out", default=None)
     args = ap.parse_args(argv)
+    if args.kernels and args.cache_type != "f16":
+        ap.error("--kernels times the fp16 cache's kernels")
     LK.gemv_impl(LK.GEMV_MFMA if args.gemv_impl == "mfma" else LK.GEMV_VALU)
     if not torch.cuda.is_available():
         print("llm_bench needs an MI355X", file=sys.stderr)
@@ -205,7 +209,7 @@ def main(argv=None) -> int:
     w = ModelWeights.random(cfg, device=dev, seed=0)
     torch.cuda.synchronize()
     ctx = args.ctx or max(4096, args.prompt + args.steps + 64)
-    eng = Engine(w, max_ctx=ctx, slots=8, dense=True)
+    eng = Engine(w, max_ctx=ctx, slots=8, dense=True, kv_type=args.cache_type)
     if args.norm_prologue_t:
         eng.norm_prologue_t = args.norm_prologue_t
     eng.dense_weights()
