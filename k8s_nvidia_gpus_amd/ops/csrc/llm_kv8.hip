@@ -996,12 +996,15 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
 }
 
 // ---------------------------------------------------------------- prompt attention
-// Rows of one KV head are token-major, row = token x G + head in group; a workgroup has NW waves of 32
-// rows.  Each page goes through LDS once for all of them, turned to fp16 on the way (double buffered;
-// the next page's loads are in flight during this one's maths).  S^T = K Q^T and O^T = V^T P^T on
-// v_mfma_f32_32x32x16_f16, a lane owns one query row: softmax and rescaling need one exchange (lane
-// ^ 32).  The key of position p lies in LDS row p with bits 2 and 3 swapped, so that the score
-// registers of a lane are, in order, the P operand's consecutive positions: P never moves.
+// Rows of one KV head are token-major, row = token x G + head in group; a workgroup has RW waves of 32
+// rows, or two slots of RW waves that take the row block's pages in turn, each through its own buffers,
+// and add up in LDS at the end (for grids too small to give a SIMD two waves otherwise: the chain of
+// pages halves, 1024 rows at 0 31 -> 26 us).  Each page goes through LDS once for all rows, turned to
+// fp16 on the way (double buffered; the next page's loads are in flight during this one's maths).
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_f16, a lane owns one query row: softmax and
+// rescaling need one exchange (lane ^ 32).  The key of position p lies in LDS row p with bits 2 and 3
+// swapped, so that the score registers of a lane are, in order, the P operand's consecutive positions: P
+// never moves.
 // What bounds it: matrix and vector instructions of a SIMD's two waves hardly overlap (8192 rows at 0:
 // matrix cores busy 42 % of the time, vector units 48 %), and half of the vector time is the exponents;
 // three waves a SIMD took 12 % fewer cycles at a clock 11 % lower.
@@ -1047,25 +1050,27 @@ __device__ __forceinline__ void image_values(char* to, int c, const uint4& v, in
   *reinterpret_cast<h8*>(to + Image<D>::value(d, ch + 1)) = codes_h8<FP8>(w[2], w[3]);
 }
 
-template <int D, bool FP8, int T, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a) {
+template <int D, bool FP8, int T, int RW, int SLOTS>
+__global__ void __launch_bounds__(64 * RW * SLOTS, 2) kv8_prompt_kernel(const AttnArgs a) {
   typedef Image<D> I;
   constexpr int KS = D / 16, DB = D / 32;
-  constexpr int NT = 64 * NW, NCH = kPage * D / 16, CH = (NCH + NT - 1) / NT;   // 16-code chunks a thread
+  constexpr int NT = 64 * RW, NCH = kPage * D / 16, CH = (NCH + NT - 1) / NT;   // 16-code chunks a thread
   constexpr int BUF = I::kKeys + I::kValues;
-  __shared__ __align__(16) char lds[2 * BUF];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ __align__(16) char shared[SLOTS * 2 * BUF];
+  const int slot = SLOTS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  const int tid = threadIdx.x - slot * NT, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  char* lds = shared + slot * 2 * BUF;
   const int r = lane & 31, hh = lane >> 5;
   const int kh = blockIdx.x % a.c.Hkv;
   // later pieces (of a causal prompt: the longest) first
   const int unit = a.units - 1 - (int)(blockIdx.x / a.c.Hkv);
   Piece pc;
-  if (!find_piece(a.sg, unit, [&](int n, int) { return (int)(((long)n * a.G + 32 * NW - 1) / (32 * NW)); }, pc))
+  if (!find_piece(a.sg, unit, [&](int n, int) { return (int)(((long)n * a.G + 32 * RW - 1) / (32 * RW)); }, pc))
     return;
   const int s = pc.s, row0 = pc.row, cnt = pc.cnt, start = pc.pos;
-  const int rows = cnt * a.G, R0 = pc.index * 32 * NW;
+  const int rows = cnt * a.G, R0 = pc.index * 32 * RW;
   const int span = min(a.span, a.c.width * kPage);
-  const int t_hi = min(cnt - 1, (R0 + 32 * NW - 1) / a.G);
+  const int t_hi = min(cnt - 1, (R0 + 32 * RW - 1) / a.G);
   const Seen seen = seen_pages(start + R0 / a.G, start + t_hi, span, a.window, a.sinks);
   const int each = (seen.n + a.parts - 1) / a.parts;
   const int t0 = min(seen.n, (int)blockIdx.y * each), t1 = min(seen.n, t0 + each);
@@ -1156,23 +1161,23 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
 
   int id = -1;
   float ks = 0.f, vs = 0.f;
-  if (t0 < t1) {
-    entry(t0, id, ks, vs);
+  int t = t0 + slot;
+  if (t < t1) {
+    entry(t, id, ks, vs);
     load_tile(id);
-    store_tile(0, end - seen.page(t0) * kPage);
+    store_tile(0, end - seen.page(t) * kPage);
   }
   __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
+  for (int buf = 0; t < t1 + slot; t += SLOTS, buf ^= 1) {   // (as many turns in every slot)
     const int base = seen.page(t) * kPage;
     int id1 = -1;
     float ks1 = 0.f, vs1 = 0.f;
-    if (t + 1 < t1) {
-      entry(t + 1, id1, ks1, vs1);
+    if (t + SLOTS < t1) {
+      entry(t + SLOTS, id1, ks1, vs1);
       load_tile(id1);
     }
     const bool hidden = base > w_hi || (a.window > 0 && base + kPage - 1 <= w_lo - a.window && base >= a.sinks);
-    if (wave_in && id >= 0 && !hidden) {
+    if (wave_in && id >= 0 && !hidden) {                 // (id is -1 behind t1)
       const char* kl = lds + buf * BUF + kfrag;
       f16v sc[2];
       const f16v zero = {};
@@ -1264,11 +1269,35 @@ __global__ void __launch_bounds__(64 * NW, 2) kv8_prompt_kernel(const AttnArgs a
               *reinterpret_cast<const h8*>(lds + buf * BUF + vfrag + 32 * st + 32 * b * I::kValueRow), pa[st], o[b],
               0, 0, 0);
     }
-    if (t + 1 < t1) store_tile(buf ^ 1, end - seen.page(t + 1) * kPage);
+    if (t + SLOTS < t1) store_tile(buf ^ 1, end - seen.page(t + SLOTS) * kPage);
     id = id1; ks = ks1; vs = vs1;
     __syncthreads();
   }
   l += xor32(l);
+  if constexpr (SLOTS == 2) {                            // the second slot's share joins the first's
+    float* to = reinterpret_cast<float*>(shared) + wave * (16 * DB + 2) * 64 + lane;
+    if (slot) {
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) to[64 * (16 * b + i)] = o[b][i] * vref;
+      to[64 * 16 * DB] = m;
+      to[64 * (16 * DB + 1)] = l;
+    }
+    __syncthreads();
+    if (slot) return;
+    const float m2 = to[64 * 16 * DB], l2 = to[64 * (16 * DB + 1)], M = fmaxf(m, m2);
+    const float e1 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+    const float e2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - M);
+    // (a NaN sum: a poisoned page, whose maximum may still be -inf)
+    l = (l != l ? l : l * e1) + (l2 != l2 ? l2 : l2 * e2);
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[b][i] = o[b][i] * vref * e1 + to[64 * (16 * b + i)] * e2;
+    m = M;
+    vref = 1.f;
+  }
   if (!valid) return;
   const long grow = (long)row0 + tok;
   if (a.parts > 1) {
@@ -1427,22 +1456,29 @@ DecodePlan decode_plan(const AttnCall& c) {
 }
 
 struct PromptPlan {
-  int nw;
+  int rw, slots;                       // waves of 32 rows, key slots
   long units, parts;
 };
-// Waves a workgroup (4 or 8, of 32 rows each) and workgroups that share a row block's pages, by what they
-// take (microseconds, measured at D 128): a page costs a workgroup 1.5 alone on its CU and 2.05 beside
-// another (4 waves: two fit), 1.95 with 8 waves (one fits); partial outputs cost a join launch and their
-// bytes.  The time is the longest row block's or that of the rounds over the chip, whichever is more; a
-// causal chunk's own pages count half, as its row blocks see them on average.
-// Both sides: 2048 rows at 0 57 (4 waves) against 67 us, 4096 at 0 144 against 132, 512 at 16000 154
-// against 142; 16 rows at 500 in 1 part 20, in 4 15, 512 rows at 0 19 against 30.
+// The workgroup's form and how many workgroups share a row block's pages, by what they take (microseconds,
+// measured at D 128): its start and end, partly hidden in rounds after the first; a page, 1.5 for 4 waves
+// alone on their CU and 2.05 beside another workgroup (two fit), 1.95 for 8 waves of rows, 1.1 for 4 of
+// rows in two key slots (of either one fits); partial outputs cost a join launch and their bytes.  The
+// time is the longest row block's or that of the rounds over the chip, whichever is more; a causal chunk's
+// own pages count half, as its row blocks see them on average.
+// The three forms without parts: 128 rows at 0 10.5, 13.8, 11.3 us; 512 at 512 30, 38, 26; 2048 at 0 58,
+// 68, 50; 4096 at 0 145, 133, 155; 6 x 300 at 700 36, 39, 41.  Parts: 16 rows at 500 in 1 part 20, in 8
+// 13; 512 rows at 0 in 1 part 19, in 2 28; 512 at 16000, 8 waves, in 1, 2, 4, 8 parts 458, 247, 138, 151.
 PromptPlan prompt_plan(const AttnCall& c) {
+  struct Form {
+    int rw, slots, fit;                // fit: workgroups on the chip
+    double base, again, page;
+  };
+  constexpr Form forms[] = {{4, 1, 512, 7.2, 2.5, 1.5}, {8, 1, 256, 9, 3.5, 1.95}, {4, 2, 256, 8.4, 6, 1.1}};
   const long G = c.heads / c.c.hkv;
-  PromptPlan best{4, 0, 1};
+  PromptPlan best{4, 1, 0, 1};
   double least = 0;
-  for (int nw = 4; nw <= 8; nw += 4) {
-    const long rows = 32 * nw, slots = nw == 8 ? 256 : 512;
+  for (const Form& f : forms) {
+    const long rows = 32 * f.rw;
     long units = c.n * G / rows + c.s;
     if (G <= rows && units > c.n) units = c.n;
     const long n = most_seen(c, (rows + G - 1) / G + 1);
@@ -1450,14 +1486,15 @@ PromptPlan prompt_plan(const AttnCall& c) {
     const double mean = n - 0.5 * (own < n ? own : n);
     const double bytes = 8.0 * c.n * c.heads * c.c.d;
     for (long p = 1; p <= n && p <= (c.n > 65535 ? 1 : 64); ++p) {   // (the join's grid has 16 bits of rows)
-      const long wgs = units * c.c.hkv * p;
+      const long wgs = units * c.c.hkv * p, rounds = (wgs + f.fit - 1) / f.fit;
       const double crowd = (wgs * mean / n - 256) / 128;  // CUs with two workgroups: none to most
-      const double page = nw == 8 ? 1.95 : 1.5 + 0.55 * (crowd < 0 ? 0 : crowd > 1 ? 1 : crowd);
-      const double longest = (double)((n + p - 1) / p) * page, all = (double)((wgs + slots - 1) / slots) * mean / p * page;
-      const double t = (longest > all ? longest : all) + (p > 1 ? 3.5 + p * bytes / 3.5e6 : 0);
+      const double page = f.page + (f.fit == 512 ? 0.55 * (crowd < 0 ? 0 : crowd > 1 ? 1 : crowd) : 0);
+      const double longest = (double)((n + p - 1) / p) * page, all = rounds * mean / p * page;
+      const double t = f.base + f.again * (rounds - 1) + (longest > all ? longest : all) +
+                       (p > 1 ? 4.5 + p * bytes / 4.5e6 : 0);
       if (best.units == 0 || t < least) {
         least = t;
-        best = {nw, units, p};
+        best = {f.rw, f.slots, units, p};
       }
     }
   }
@@ -1599,13 +1636,18 @@ int amdk8s_llm_kv8_prompt(const void* call, float scale, void* work, long work_f
   return by_format(c.c, [&](auto d, auto f) -> int {
     constexpr int DD = decltype(d)::value;
     constexpr bool F8 = decltype(f)::value;
-    auto go = [&](auto nw) {
-      constexpr int NW = decltype(nw)::value;
-      if (c.type == kF16) hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kF16, NW>), grid, dim3(64 * NW), 0, st, a);
-      else hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kBF16, NW>), grid, dim3(64 * NW), 0, st, a);
+    auto go = [&](auto rw, auto slots) {
+      constexpr int RW = decltype(rw)::value, SL = decltype(slots)::value;
+      if (c.type == kF16) hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kF16, RW, SL>), grid, dim3(64 * RW * SL), 0, st, a);
+      else hipLaunchKernelGGL((kv8_prompt_kernel<DD, F8, kBF16, RW, SL>), grid, dim3(64 * RW * SL), 0, st, a);
     };
-    if (plan.nw == 8) go(std::integral_constant<int, 8>{});
-    else go(std::integral_constant<int, 4>{});
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I4 = std::integral_constant<int, 4>;
+    using I8 = std::integral_constant<int, 8>;
+    if (plan.slots == 2) go(I4{}, I2{});
+    else if (plan.rw == 8) go(I8{}, I1{});
+    else go(I4{}, I1{});
     if (need) {
       const dim3 rows((unsigned)c.heads, (unsigned)c.n);
       if (c.type == kF16) hipLaunchKernelGGL((kv8_join_kernel<DD, kF16, 1, false>), rows, dim3(64), 0, st, a);

@@ -482,6 +482,44 @@ def test_prompt_ignores_what_lies_behind_a_chunk(KV):
     assert torch.equal(run_prompt(KV, cache, rows, q, starts, lens), want)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 70), (64, 0), (1, 1)])
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("h,hkv,d,dtype", [(28, 4, 128, torch.float16), (8, 4, 64, torch.bfloat16)])
+def test_prompt_of_middling_grids(KV, window, sinks, code, h, hkv, d, dtype):
+    """Grids between a quarter and all of the chip, odd and even numbers of pages: unmapped pages, dead rows
+    full of NaN codes, value scales from page to page, a sequence without rows and rows behind the last."""
+    starts, lens = [480, 333, 0, 0, 1000], [500, 130, 0, 190, 65]
+    cache, rows, q = prompt_case(KV, starts, lens, h, hkv, d, code, dtype, seed=70, pad=3)
+    e = torch.randint(-12, 13, cache.vs.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(71))
+    cache.vs.copy_(torch.exp2(e.double() - 6))
+    for s, i in ((0, 3), (0, 10), (1, 0), (4, 15)):
+        rows[s][i] = -1
+    if code == "e4m3":
+        for s in (0, 1, 3, 4):
+            n = starts[s] + lens[s]
+            if n % PAGE:
+                bits(cache.k)[rows[s][n // PAGE], :, n % PAGE:] = 0x7f
+                bits(cache.v)[rows[s][n // PAGE], :, :, n % PAGE:] = 0xff
+    got = run_prompt(KV, cache, rows, q, starts, lens, window=window, sinks=sinks)
+    if code == "e4m3":                                       # (the plain form would meet the NaNs)
+        dead = bits(cache.v) & 0x7f == 0x7f
+        bits(cache.v)[dead] = 0
+        bits(cache.k)[bits(cache.k) & 0x7f == 0x7f] = 0
+    check_prompt(cache, rows, q, starts, lens, got, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("n", [960, 1000])
+def test_prompt_of_a_middling_grid_with_poisoned_pages(KV, n):
+    cache, rows, q = prompt_case(KV, [0], [n], 28, 4, 128, "int8", torch.float16, seed=72)
+    clean = run_prompt(KV, cache, rows, q, [0], [n])
+    for i, t in ((6, cache.ks), (9, cache.vs)):
+        old = t[rows[0][i]].clone()
+        t[rows[0][i]] = float("nan")
+        got = run_prompt(KV, cache, rows, q, [0], [n])
+        assert torch.equal(got[:i * PAGE], clean[:i * PAGE]) and got[i * PAGE:].isnan().all()
+        t[rows[0][i]] = old
+
+
 def test_prompt_pages_of_unlike_scales(KV):
     starts, lens = [0, 400], [300, 100]
     cache, rows, q = prompt_case(KV, starts, lens, 8, 2, 128, "int8", torch.bfloat16, seed=5)
