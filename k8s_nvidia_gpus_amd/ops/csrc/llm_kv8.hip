@@ -1400,6 +1400,11 @@ bool good_attn(const AttnCall& c) {
   return good_pool(c.c) && c.start && c.q.at && in(c.heads, 1, 0x3fffffff) && c.heads % c.c.hkv == 0 &&
          in(c.type, 0, 1) && in(c.span, 1, c.c.width * kPage) && in(c.window, 0, 1 << 30) && in(c.sinks, 0, 1 << 30);
 }
+bool good_decode(const AttnCall& c) { return good_attn(c) && in(c.s, 1, 65535) && c.n == c.s; }
+bool good_prompt(const AttnCall& c) {
+  return good_attn(c) && good_segs(c.start, c.cu, c.s, c.n) && c.n * (c.heads / c.c.hkv) <= 0x3fffffffL;
+}
+long work_floats_of(const AttnCall& c, long parts) { return parts == 1 ? 0 : parts * c.n * c.heads * (c.c.d + 2); }
 AttnArgs make_attn(const AttnCall& c, float scale, void* work, long parts) {
   AttnArgs a{};
   a.c = make_pool(c.c);
@@ -1486,12 +1491,13 @@ PromptPlan prompt_plan(const AttnCall& c) {
     const double mean = n - 0.5 * (own < n ? own : n);
     const double bytes = 8.0 * c.n * c.heads * c.c.d;
     for (long p = 1; p <= n && p <= (c.n > 65535 ? 1 : 64); ++p) {   // (the join's grid has 16 bits of rows)
+      const double join = p > 1 ? 4.5 + p * bytes / 4.5e6 : 0;
+      if (best.units && f.base + join > least) break;
       const long wgs = units * c.c.hkv * p, rounds = (wgs + f.fit - 1) / f.fit;
       const double crowd = (wgs * mean / n - 256) / 128;  // CUs with two workgroups: none to most
       const double page = f.page + (f.fit == 512 ? 0.55 * (crowd < 0 ? 0 : crowd > 1 ? 1 : crowd) : 0);
       const double longest = (double)((n + p - 1) / p) * page, all = rounds * mean / p * page;
-      const double t = f.base + f.again * (rounds - 1) + (longest > all ? longest : all) +
-                       (p > 1 ? 4.5 + p * bytes / 4.5e6 : 0);
+      const double t = f.base + f.again * (rounds - 1) + (longest > all ? longest : all) + join;
       if (best.units == 0 || t < least) {
         least = t;
         best = {f.rw, f.slots, units, p};
@@ -1576,19 +1582,17 @@ int amdk8s_llm_kv8_read(const void* call, void* stream) {
 // fp32 workspace (in floats) of the call: 0 when its partials need no join, -1 for a bad argument
 long amdk8s_llm_kv8_decode_work(const void* call) {
   const AttnCall& c = *static_cast<const AttnCall*>(call);
-  if (!good_attn(c) || !in(c.s, 1, 65535) || c.n != c.s) return -1;
-  const long parts = decode_plan(c).parts;
-  return parts == 1 ? 0 : parts * c.n * c.heads * (c.c.d + 2);
+  return good_decode(c) ? work_floats_of(c, decode_plan(c).parts) : -1;
 }
 
 // One query row a sequence at position start[s] (-1: nothing to see, zeros); keys at or behind `span` are
 // not attended.
 int amdk8s_llm_kv8_decode(const void* call, float scale, void* work, long work_floats, void* stream) {
   const AttnCall& c = *static_cast<const AttnCall*>(call);
-  const long need = amdk8s_llm_kv8_decode_work(call);
-  if (need < 0 || need > work_floats || (need && (!work || ((uintptr_t)work & 15)))) return 2;
-  if ((!c.out.at && !c.x8) || (c.x8 && (!c.dx || !c.sx))) return 2;
+  if (!good_decode(c) || (!c.out.at && !c.x8) || (c.x8 && (!c.dx || !c.sx))) return 2;
   const DecodePlan plan = decode_plan(c);
+  const long need = work_floats_of(c, plan.parts);
+  if (need > work_floats || (need && (!work || ((uintptr_t)work & 15)))) return 2;
   if (plan.parts > 65535) return 2;
   AttnArgs a = make_attn(c, scale, need ? work : nullptr, plan.parts);
   a.per = plan.per;
@@ -1615,19 +1619,17 @@ int amdk8s_llm_kv8_decode(const void* call, float scale, void* work, long work_f
 
 long amdk8s_llm_kv8_prompt_work(const void* call) {
   const AttnCall& c = *static_cast<const AttnCall*>(call);
-  if (!good_attn(c) || !good_segs(c.start, c.cu, c.s, c.n) || c.n * (c.heads / c.c.hkv) > 0x3fffffffL) return -1;
-  const long parts = prompt_plan(c).parts;
-  return parts == 1 ? 0 : parts * c.n * c.heads * (c.c.d + 2);
+  return good_prompt(c) ? work_floats_of(c, prompt_plan(c).parts) : -1;
 }
 
 // Query rows of the segments (row cu[s] + i at position start[s] + i) over the cache, their own keys
 // included; rows in no segment are left as they are.
 int amdk8s_llm_kv8_prompt(const void* call, float scale, void* work, long work_floats, void* stream) {
   const AttnCall& c = *static_cast<const AttnCall*>(call);
-  const long need = amdk8s_llm_kv8_prompt_work(call);
-  if (need < 0 || need > work_floats || (need && (!work || ((uintptr_t)work & 15)))) return 2;
-  if (!c.out.at || c.x8) return 2;
+  if (!good_prompt(c) || !c.out.at || c.x8) return 2;
   const PromptPlan plan = prompt_plan(c);
+  const long need = work_floats_of(c, plan.parts);
+  if (need > work_floats || (need && (!work || ((uintptr_t)work & 15)))) return 2;
   if (plan.units * c.c.hkv > 0x7fffffffL || plan.parts > 65535 || (plan.parts > 1 && c.n > 65535)) return 2;
   AttnArgs a = make_attn(c, scale, need ? work : nullptr, plan.parts);
   a.units = (int)plan.units;

@@ -99,31 +99,32 @@ def _bad(what: str, why: str):
 def _pool(what: str, cache: Sequence[torch.Tensor], pages: torch.Tensor):
     """Checked cache and table -> (device index, Hkv, D, sequences, columns, the record's fields)."""
     k, v, ks, vs = cache
-    shape, code = k.shape, k.dtype
-    if len(shape) != 4 or code not in _CODES or v.dtype != code or shape[2] != PAGE \
+    shape, kind = k.shape, k.dtype
+    code = _CODES.get(kind)
+    if code is None or len(shape) != 4 or v.dtype is not kind or shape[2] != PAGE \
             or shape[3] not in (64, 128) or v.shape != (shape[0], shape[1], shape[3], PAGE) \
             or not k.is_contiguous() or not v.is_contiguous() or shape[0] < 1 or shape[1] < 1:
-        _bad(what, f"cache codes k {tuple(shape)} {code}, v {tuple(v.shape)} {v.dtype} are not "
+        _bad(what, f"cache codes k {tuple(shape)} {kind}, v {tuple(v.shape)} {v.dtype} are not "
                    f"contiguous [pages, Hkv, {PAGE}, D] and [pages, Hkv, D, {PAGE}] of int8 or "
                    f"float8_e4m3fn with D 64 or 128")
     n, hkv, _, d = shape
     dev, each = k.get_device(), (n, hkv)
-    if ks.dtype != _F32 or ks.shape != each or not ks.is_contiguous() or ks.get_device() != dev \
-            or vs.dtype != _F32 or vs.shape != each or not vs.is_contiguous() or vs.get_device() != dev:
+    if ks.dtype is not _F32 or ks.shape != each or not ks.is_contiguous() or ks.get_device() != dev \
+            or vs.dtype is not _F32 or vs.shape != each or not vs.is_contiguous() or vs.get_device() != dev:
         _bad(what, f"scales must be contiguous fp32 [{n}, {hkv}] on {k.device}")
     if v.get_device() != dev:
         _bad(what, f"the cache must lie on one device, not {k.device} / {v.device}")
     table, strides = pages.shape, pages.stride()
-    if pages.dtype != _I32 or len(table) != 2 or table[0] < 1 or table[1] < 1 or strides[1] != 1 \
+    if pages.dtype is not _I32 or len(table) != 2 or table[0] < 1 or table[1] < 1 or strides[1] != 1 \
             or pages.get_device() != dev:
         _bad(what, f"the page table must be int32 [S, columns] with a unit inner stride on {k.device}")
     return dev, hkv, d, table[0], table[1], (
         k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages.data_ptr(), n, hkv, d,
-        _CODES[code], table[1], strides[0])
+        code, table[1], strides[0])
 
 
 def _ints(what: str, name: str, t: torch.Tensor, n: int, dev: int) -> int:
-    if t.dtype != _I32 or t.shape != (n,) or not t.is_contiguous() or t.get_device() != dev:
+    if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous() or t.get_device() != dev:
         _bad(what, f"{name} must be contiguous int32 [{n}] on the cache's device")
     return t.data_ptr()
 
@@ -141,6 +142,8 @@ def _out_rows(what: str, name: str, t: torch.Tensor, n: int, heads: int, d: int,
     """`_rows` of an output: its rows must not share memory (an expanded view would)."""
     rows = _rows(what, name, t, n, heads, d, dev)
     _, row, head = rows
+    if head >= d and row >= heads * head:
+        return rows
     if (heads > 1 and head < d) or (n > 1 and row < d) \
             or (n > 1 and heads > 1 and row < (heads - 1) * head + d and head < (n - 1) * row + d):
         _bad(what, f"{name} {tuple(t.shape)} / {t.stride()}: its rows overlap")
@@ -153,7 +156,7 @@ def _gpu(what: str, dev: int) -> None:
 
 
 def _launch(what: str, dev: int, fn, *args) -> None:
-    if dev != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():                # (a tensor there: the runtime is up)
         with torch.cuda.device(dev):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
