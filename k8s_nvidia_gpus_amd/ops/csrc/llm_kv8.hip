@@ -511,7 +511,7 @@ struct ReadArgs {
 };
 
 // One page of one sequence and KV head a block: keys row by row, values through byte transposes and LDS.
-// Memory-bound, two thirds of it the values' stores: 8 x 16384 positions 68 us, 4.3 TB/s.
+// Memory-bound, four fifths of the bytes stores: 8 x 16384 positions 68 us, 4.3 TB/s.
 template <int D, bool FP8, int T>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
   typedef typename Elem<T>::type E;
@@ -698,8 +698,8 @@ __device__ __forceinline__ void put_q8(const AttnArgs& a, int t, long col, const
 // A page's keys are loaded as soon as the last page's have been used, and its values likewise: 16 KB in
 // flight a wave most of the time at half the registers of two buffers, so three waves fit a SIMD (two
 // buffers left one; 32 x 16000 with a window 140 us, this 61).  Bound by the cache's bytes: 8 x 32768
-// in e4m3 45 us, 4.7 TB/s, where a copy reaches 5.1; short contexts by launches (two, 2 to 3 us each) and
-// the chain position, page entry, page, join: 8 x 4096 13.4 us, 500 positions 8.1.
+// in e4m3 44 us, 4.8 TB/s, where a copy reaches 5.1; short contexts by launches (two, 2 to 3 us each) and
+// the chain position, page entry, page, join: 8 x 4096 13.3 us, 500 positions 8.1.
 template <int D, bool FP8, int T, int NW>
 __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a) {
   constexpr int KH = D / 64, ND = D / 16;
@@ -1008,7 +1008,7 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
 // What bounds it: matrix and vector instructions of a SIMD's two waves hardly overlap (8192 rows at 0:
 // matrix cores busy 42 % of the time, vector units 48 %), and half of the vector time is the exponents;
 // three waves a SIMD took 12 % fewer cycles at a clock 11 % lower.
-// 8192 at 0 500 us, 960 TFLOP/s of visible pairs (a library product of two 8192 matrices reaches 1450);
+// 8192 at 0 496 us, 970 TFLOP/s of visible pairs (a library product of two 8192 matrices reaches 1450);
 // 512 at 31488 250 us.  Tried and not taken: 64 rows a wave (twice the registers, one wave a SIMD: 660
 // us), the next page's scores ahead of this page's weights (580), pages turned to fp16 images in memory
 // once and loaded into LDS directly (503, and 284 for 512 at 31488), wave priorities (no change).
