@@ -55,6 +55,13 @@ struct Elem<kF32> {
   static __device__ __forceinline__ float put(float x) { return x; }
 };
 
+// 16 bytes that nobody reads again soon: non-temporal, so that they leave the caches to others.  Only where
+// an instruction takes whole 128-byte lines; the rest of a line in pieces is fetched again.
+typedef unsigned u4v __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 load16_once(const void* p) {
+  return __builtin_bit_cast(uint4, __builtin_nontemporal_load(static_cast<const u4v*>(p)));
+}
+
 // N consecutive elements as floats; `wide`: the address is a multiple of 16 bytes (uniform)
 template <int T, int N>
 __device__ __forceinline__ void load_n(const typename Elem<T>::type* p, bool wide, float (&x)[N]) {
@@ -74,7 +81,8 @@ __device__ __forceinline__ void load_n(const typename Elem<T>::type* p, bool wid
     for (int i = 0; i < N; ++i) x[i] = Elem<T>::get(p[i]);
   }
 }
-template <int T, int N>
+// ONCE: non-temporal
+template <int T, int N, bool ONCE = false>
 __device__ __forceinline__ void store_n(typename Elem<T>::type* p, bool wide, const float (&x)[N]) {
   typedef typename Elem<T>::type E;
   constexpr int PER = 16 / sizeof(E);
@@ -84,9 +92,10 @@ __device__ __forceinline__ void store_n(typename Elem<T>::type* p, bool wide, co
       E e[PER];
 #pragma unroll
       for (int i = 0; i < PER; ++i) e[i] = Elem<T>::put(x[c * PER + i]);
-      uint4 w;
+      u4v w;
       __builtin_memcpy(&w, e, 16);
-      reinterpret_cast<uint4*>(p)[c] = w;
+      if constexpr (ONCE) __builtin_nontemporal_store(w, reinterpret_cast<u4v*>(p) + c);
+      else reinterpret_cast<u4v*>(p)[c] = w;
     }
   } else {
 #pragma unroll
@@ -511,7 +520,8 @@ struct ReadArgs {
 };
 
 // One page of one sequence and KV head a block: keys row by row, values through byte transposes and LDS.
-// Memory-bound, four fifths of the bytes stores: 8 x 16384 positions 68 us, 4.3 TB/s.
+// Memory-bound, four fifths of the bytes stores: 8 x 16384 positions 56 us, 5.1 TB/s; through the caches
+// (key codes in, rows out) 68.
 template <int D, bool FP8, int T>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
   typedef typename Elem<T>::type E;
@@ -534,7 +544,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
   const uint32_t mask = live ? ~0u : 0u;
   uint4 kx[PK];
 #pragma unroll
-  for (int u = 0; u < PK; ++u) kx[u] = reinterpret_cast<const uint4*>(kc)[tid + 256 * u];
+  for (int u = 0; u < PK; ++u) kx[u] = load16_once(kc + 16 * (tid + 256 * u));
   uint2 vx[PV][4];                                       // 8 positions of 4 dims
 #pragma unroll
   for (int u = 0; u < PV; ++u)
@@ -551,7 +561,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[4 * c + e] = x[e] * scale;
     }
-    store_n<T, 16>(out, a.wide, y);
+    store_n<T, 16, true>(out, a.wide, y);
   };
 #pragma unroll
   for (int u = 0; u < PK; ++u) {
@@ -697,10 +707,12 @@ __device__ __forceinline__ void put_q8(const AttnArgs& a, int t, long col, const
 //   maximum, sum and rescaling are one head's, a lane's own.
 // A page's keys are loaded as soon as the last page's have been used, and its values likewise: 16 KB in
 // flight a wave most of the time at half the registers of two buffers, so three waves fit a SIMD (two
-// buffers left one; 32 x 16000 with a window 140 us, this 61).  Bound by the cache's bytes: 8 x 32768
-// in e4m3 44 us, 4.8 TB/s, where a copy reaches 5.1; short contexts by launches (two, 2 to 3 us each) and
-// the chain position, page entry, page, join: 8 x 4096 13.3 us, 500 positions 8.1.
-template <int D, bool FP8, int T, int NW>
+// buffers left one; 32 x 16000 with a window 140 us, this 61).  ONCE: up to 16 heads a KV head, so that no
+// other workgroup reads the page; its values are loaded past the caches (8 x 32768 44 -> 40 us, with the
+// window 61 -> 57; with 128 heads on one KV head 14.5 -> 16.6).  Bound by the cache's bytes: 8 x 32768 in
+// e4m3 40 us, 5.2 TB/s, where a copy reaches 5.1; short contexts by launches (two, 2 to 3 us each) and the
+// chain position, page entry, page, join: 8 x 4096 13.4 us, 500 positions 8.1.
+template <int D, bool FP8, int T, int NW, bool ONCE>
 __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a) {
   constexpr int KH = D / 64, ND = D / 16;
   const int hg = (a.G + 15) / 16;
@@ -745,7 +757,8 @@ __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a
     const long id = max(__builtin_amdgcn_readlane(my_id, i), 0);
     const uint8_t* vp = a.c.v + (id * a.c.Hkv + kh) * (kPage * D) + pr * kPage + 16 * kg;
 #pragma unroll
-    for (int n = 0; n < ND; ++n) vr[n] = *reinterpret_cast<const uint4*>(vp + 16 * n * kPage);
+    for (int n = 0; n < ND; ++n)
+      vr[n] = ONCE ? load16_once(vp + 16 * n * kPage) : *reinterpret_cast<const uint4*>(vp + 16 * n * kPage);
   };
   if (mine > 0) {
     load_keys(0);
@@ -1601,13 +1614,17 @@ int amdk8s_llm_kv8_decode(const void* call, float scale, void* work, long work_f
   return by_format(c.c, [&](auto d, auto f) -> int {
     constexpr int DD = decltype(d)::value;
     constexpr bool F8 = decltype(f)::value;
-    auto go = [&](auto nw) {
+    auto go = [&](auto nw, auto once) {
       constexpr int NW = decltype(nw)::value;
-      if (c.type == kF16) hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kF16, NW>), grid, dim3(64 * NW), 0, st, a);
-      else hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kBF16, NW>), grid, dim3(64 * NW), 0, st, a);
+      constexpr bool ON = decltype(once)::value;
+      if (c.type == kF16) hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kF16, NW, ON>), grid, dim3(64 * NW), 0, st, a);
+      else hipLaunchKernelGGL((kv8_decode_kernel<DD, F8, kBF16, NW, ON>), grid, dim3(64 * NW), 0, st, a);
     };
-    if (plan.nw == 8) go(std::integral_constant<int, 8>{});
-    else go(std::integral_constant<int, 4>{});
+    using I4 = std::integral_constant<int, 4>;
+    using I8 = std::integral_constant<int, 8>;
+    if (plan.nw == 8) go(I8{}, std::false_type{});
+    else if (a.G <= 16) go(I4{}, std::true_type{});
+    else go(I4{}, std::false_type{});
     if (need) {
       const dim3 rows((unsigned)c.heads, (unsigned)c.s);
       if (c.type == kF16) hipLaunchKernelGGL((kv8_join_kernel<DD, kF16, 4, true>), rows, dim3(256), 0, st, a);
