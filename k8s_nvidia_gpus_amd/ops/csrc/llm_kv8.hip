@@ -1447,30 +1447,35 @@ long most_seen(const AttnCall& c, long rows) {
   return w < n ? w : n;
 }
 
-constexpr long kDecodeGrid = 512;                        // workgroups: two on each of the 256 CUs
-
 struct DecodePlan {
   int nw, per;
   long parts;
 };
-// Workgroups that share a row's pages: as many as let 512 workgroups, two on each CU, take all rows in one
-// round (8 x 32768 44 us; at most 384 49; 576 and more, a second round, 48; 32 x 16000 in 4 parts 98, in
+// Workgroups that share a row's pages: as many as let all of them run in one round, 512 of 4 waves, two on
+// each CU (8 x 32768 44 us; at most 384 49; 576 and more, a second round, 48; 32 x 16000 in 4 parts 98, in
 // 5 112).  At most 64, past which the join costs what the shorter chains save (1 x 32768 in 64 parts 13.9,
 // in 128 16.0), unless a wave would have more than the 64 pages whose table entries it holds.  Where one
 // part fills the CUs, a wave has 4 pages before there is a second one (64 x 1000 in one part 14.7, in two
-// 18.5); where it does not, one page is enough (1 x 4000 with one page a wave 9.1, with two 10.7).  Up to
-// 8 pages run in one workgroup of 8 waves, which needs no join: 500 positions 8.1 us against 9.2.
+// 18.5); where it does not, one page is enough (1 x 4000 with one page a wave 9.1, with two 10.7).
+// Waves that would have two pages or more go 8 to a workgroup and half as many parts, if those fill three
+// quarters of the CUs: fewer partials (32 x 16000 with a window 57 -> 51, 64 x 4000 49 -> 45, 48 x 2000
+// 25 -> 20; with 160 of 256 CUs 60 -> 61; with one page a wave 9.2 -> 10.8).  Up to 8 pages run in one
+// workgroup of 8 waves, which needs no join: 500 positions 8.1 us against 9.2.
 DecodePlan decode_plan(const AttnCall& c) {
   const long n = most_seen(c, 1);
   if (n <= 8) return {8, 1, 1};
   const long chains = c.s * c.c.hkv * ((c.heads / c.c.hkv + 15) / 16);
-  const long fill = kDecodeGrid / chains, few = chains >= kDecodeGrid / 2 ? 4 : 1;
-  const long worth = (n + 4 * few - 1) / (4 * few), need = (n + 255) / 256;
-  long parts = fill > 64 ? 64 : fill;
-  parts = parts > worth ? worth : parts;
-  parts = parts < need ? need : parts;
-  const long per = (n + 4 * parts - 1) / (4 * parts);
-  return {4, (int)per, (n + 4 * per - 1) / (4 * per)};
+  auto plan = [&](int nw, long grid) -> DecodePlan {
+    const long fill = grid / chains, few = chains >= grid / 2 ? 16 / nw : 1;
+    const long worth = (n + nw * few - 1) / (nw * few), need = (n + 64 * nw - 1) / (64 * nw);
+    long parts = fill > 64 ? 64 : fill;
+    parts = parts > worth ? worth : parts;
+    parts = parts < need ? need : parts;
+    const long per = (n + nw * parts - 1) / (nw * parts);
+    return {nw, (int)per, (n + nw * per - 1) / (nw * per)};
+  };
+  const DecodePlan four = plan(4, 512);
+  return four.per > 1 && chains <= 256 && 256 / chains * chains >= 192 ? plan(8, 256) : four;
 }
 
 struct PromptPlan {
@@ -1622,9 +1627,8 @@ int amdk8s_llm_kv8_decode(const void* call, float scale, void* work, long work_f
     };
     using I4 = std::integral_constant<int, 4>;
     using I8 = std::integral_constant<int, 8>;
-    if (plan.nw == 8) go(I8{}, std::false_type{});
-    else if (a.G <= 16) go(I4{}, std::true_type{});
-    else go(I4{}, std::false_type{});
+    if (a.G > 16) plan.nw == 8 ? go(I8{}, std::false_type{}) : go(I4{}, std::false_type{});
+    else plan.nw == 8 ? go(I8{}, std::true_type{}) : go(I4{}, std::true_type{});
     if (need) {
       const dim3 rows((unsigned)c.heads, (unsigned)c.s);
       if (c.type == kF16) hipLaunchKernelGGL((kv8_join_kernel<DD, kF16, 4, true>), rows, dim3(256), 0, st, a);
