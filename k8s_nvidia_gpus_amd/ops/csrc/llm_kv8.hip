@@ -707,11 +707,11 @@ __device__ __forceinline__ void put_q8(const AttnArgs& a, int t, long col, const
 //   maximum, sum and rescaling are one head's, a lane's own.
 // A page's keys are loaded as soon as the last page's have been used, and its values likewise: 16 KB in
 // flight a wave most of the time at half the registers of two buffers, so three waves fit a SIMD (two
-// buffers left one; 32 x 16000 with a window 140 us, this 61, with what follows 51).  ONCE: up to 16 heads a KV head, so that no
-// other workgroup reads the page; its values are loaded past the caches (8 x 32768 44 -> 40 us, with the
-// window 61 -> 57; with 128 heads on one KV head 14.5 -> 16.6).  Bound by the cache's bytes: 8 x 32768 in
-// e4m3 40 us, 5.2 TB/s, where a copy reaches 5.1; short contexts by launches (two, 2 to 3 us each) and the
-// chain position, page entry, page, join: 8 x 4096 13.4 us, 500 positions 8.1.
+// buffers left one; 32 x 16000 with a window 140 us, this 61, with what follows 51).  ONCE: up to 16 heads
+// a KV head, so that no other workgroup reads the page; its values are loaded past the caches (8 x 32768
+// 44 -> 40 us, with the window 61 -> 57; with 128 heads on one KV head 14.5 -> 16.6).  Bound by the cache's
+// bytes: 8 x 32768 in e4m3 40 us, 5.2 TB/s, where a copy reaches 5.1; short contexts by launches (two, 2 to
+// 3 us each) and the chain position, page entry, page, join: 8 x 4096 13.4 us, 500 positions 8.1.
 template <int D, bool FP8, int T, int NW, bool ONCE>
 __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a) {
   constexpr int KH = D / 64, ND = D / 16;

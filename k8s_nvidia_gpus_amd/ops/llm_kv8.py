@@ -14,7 +14,8 @@ a sliding window has left behind can be freed.
 
 Both attentions take a sliding window and a number of first positions that stay visible (sinks): the
 query at position p sees key j when ``j <= p and (window == 0 or j > p - window or j < sinks)``.  A row
-that sees nothing is zero.
+that sees nothing is zero.  Softmax weights are rounded to fp16 after the value scales have been put on
+them, relative to the largest scale that the row sees: a value 2^-25 of the largest or less adds nothing.
 
 Ragged sequences: ``cu`` (int32 [S + 1]) has the first row of each sequence, ``start`` (int32 [S]) its
 first position; rows at or behind ``cu[S]`` belong to none and their outputs stay as they were.  Lengths,
@@ -74,7 +75,8 @@ def _lib():
 class KV8Cache(NamedTuple):
     """A pool of pages.  Codes are int8 or e4m3; ``ks`` / ``vs`` are powers of two: the least that bring
     the block's largest magnitude to at most 127 (int8) or 448 (e4m3), 0 for an all-zero block and NaN
-    for one that got a non-finite value (what reads it is NaN until the page is begun anew)."""
+    for one that got a non-finite value (what reads it is NaN until the page is begun anew).  The codes of
+    appended positions are finite; the attentions count on it."""
     k: torch.Tensor       # codes [pages, Hkv, 64, D]
     v: torch.Tensor       # codes [pages, Hkv, D, 64]
     ks: torch.Tensor      # fp32 [pages, Hkv]
