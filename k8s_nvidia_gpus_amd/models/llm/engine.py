@@ -134,10 +134,15 @@ class Engine:
         # the 8-bit cache's kernels run on the GPU; the CPU reference maths rounds nothing
         self.kv_type = kv_type
         self.kv8 = None                  # 8-bit cache: one KV8Cache for each layer
+        # A sequence cut back may be continued at multiples of this many positions.  A page of the 8-bit
+        # cache that is entered in its middle keeps its scale, and that scale (or poison) may come from the
+        # positions that were cut off; a page begun anew forgets them.
+        self.prefix_step = 1
         if kv_type != "f16" and self.gpu:
             from k8s_nvidia_gpus_amd.ops import llm_kv8 as KV
 
             self.KV = KV
+            self.prefix_step = KV.PAGE
             each = self.max_ctx // KV.PAGE               # max_ctx is a multiple of 256
             self.kv8 = [KV.KV8Cache.empty(slots * each, c.kv_heads, c.head_dim, KV8_TYPES[kv_type],
                                           self.device) for _ in range(c.layers)]

@@ -39,6 +39,8 @@ sample fails gets that error, and no handler waits longer than ``--timeout`` sec
 Prompt caching (llama-server's ``cache_prompt``, on by default): every slot remembers which tokens
 its KV cache holds; a new request goes to the free slot sharing the longest prefix with its
 prompt, and only the rest of the prompt is prefilled (multi-turn chats re-send the whole history).
+With an 8-bit cache the reused prefix ends at a page (64 positions): a page continued in its middle
+would keep the scale that the dropped tokens gave it.
 As with llama-server, a reused prefix was computed in another prefill (a GEMM of another M), so
 the logits can differ in the last bits from an uncached prefill of the same prompt.  Prompts
 admitted in the same iteration are prefilled together (one GEMM over all their rows), so the same
@@ -399,11 +401,12 @@ class Scheduler:
                 self._fail(job, e)
                 continue
             # reuse the slot's KV for the shared prefix; at least one token is prefilled (its
-            # logits are the first sample)
+            # logits are the first sample), and the cut falls on a step of the engine's cache
             n_past = 0
             if job.cache_prompt:
                 n_past = min(common_prefix(self.slot_tokens.get(slot, []), job.ids),
                              len(job.ids) - 1)
+                n_past -= n_past % getattr(self.engine, "prefix_step", 1)
             self.slot_tokens[slot] = []                 # the KV is being rewritten
             job.slot, job.pos, job.n_cached = slot, n_past, n_past
             self.active[slot] = job
