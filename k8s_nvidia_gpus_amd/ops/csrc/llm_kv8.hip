@@ -635,7 +635,8 @@ __device__ __forceinline__ float score_factor(float ks, float c) {
   const float f = ks * c;
   return f < 1e-37f ? 1e-37f : f;
 }
-// log2 of a page's value scale over the reference `vref` (the largest so far, > 0 unless all were 0).
+// log2 of a page's value scale over the reference `vref` (the largest that the row has seen, > 0 unless all
+// were 0).
 // The weights p = 2^(s - m) go to the matrix instruction as fp16 p vs / vref, so that pages of unlike
 // scales add up in one accumulator; the sum of the plain p's takes the factor back (`back`).  A zero
 // page has zero codes: any weight will do.  A NaN scale stays.  What the rounding costs: 2^-12 of a
@@ -643,8 +644,8 @@ __device__ __forceinline__ float score_factor(float ks, float c) {
 // The reference maximum lies up to 8 below the true one (rescaling is put off that long) and kBias above
 // the exponent's: weights reach from 2^15, under fp16's largest, down to 2^-31 of the largest's step.
 constexpr float kDefer = 8.f, kBias = 7.f;
-__device__ __forceinline__ float value_weight(float vs, float vref, float& back) {
-  float lw = vs == 0.f ? 0.f : __builtin_amdgcn_logf(vs / vref);
+__device__ __forceinline__ float value_weight(float vs, float ratio, float& back) {   // ratio: vs / vref
+  float lw = vs == 0.f ? 0.f : __builtin_amdgcn_logf(ratio);
   lw = lw < -60.f ? -60.f : lw;                          // no fp16 weight is left there anyway
   back = __builtin_amdgcn_exp2f(-lw);
   return lw;
@@ -869,7 +870,7 @@ __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a
       }
     }
     float back;
-    const float lw = value_weight(vs, vref, back) + (m == -INFINITY ? kBias : kBias - m);
+    const float lw = value_weight(vs, vs / vref, back) + (m == -INFINITY ? kBias : kBias - m);
     h8 pa[2];
     float ls = 0.f;
 #pragma unroll
@@ -1191,6 +1192,22 @@ __global__ void __launch_bounds__(64 * RW * SLOTS, 2) kv8_prompt_kernel(const At
     }
     const bool hidden = base > w_hi || (a.window > 0 && base + kPage - 1 <= w_lo - a.window && base >= a.sinks);
     if (wave_in && id >= 0 && !hidden) {                 // (id is -1 behind t1)
+      // The reference scale is the row's own: its neighbours may see other pages, and weights relative to a
+      // larger scale that only those see would be lost.  Ahead of the matrix instructions, which hide most of
+      // it (8192 at 0 497 us with one reference for the wave, 503 so, 531 behind the masks), and by the
+      // reciprocal, exact for powers of two (508 with a division).
+      const bool poisoned = ks != ks || vs != vs;
+      const int top = min(min(pos, end - 1), base + kPage - 1);             // the row's last key of the page
+      const bool sees = top >= base && (a.window <= 0 || top > pos - a.window || base < a.sinks);
+      const float own = sees && !poisoned ? vs : 0.f;
+      if (__ballot(own > vref) != 0) {
+        const float q = own > vref ? vref / own : 1.f;
+#pragma unroll
+        for (int b = 0; b < DB; ++b) o[b] *= q;
+        vref = fmaxf(vref, own);
+      }
+      float back;
+      const float vw = value_weight(own, own * __builtin_amdgcn_rcpf(vref), back);
       const char* kl = lds + buf * BUF + kfrag;
       f16v sc[2];
       const f16v zero = {};
@@ -1208,7 +1225,6 @@ __global__ void __launch_bounds__(64 * RW * SLOTS, 2) kv8_prompt_kernel(const At
         if (st + AHEAD < KS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);                  // matrix instructions
       }
-      const bool poisoned = ks != ks || vs != vs;
       const float f = score_factor(poisoned ? 0.f : ks, qf);
       const bool whole = base + kPage - 1 <= w_lo && base + kPage <= end &&
                          (a.window <= 0 || base > w_hi - a.window || base + kPage <= a.sinks);
@@ -1229,12 +1245,6 @@ __global__ void __launch_bounds__(64 * RW * SLOTS, 2) kv8_prompt_kernel(const At
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
       mx *= f;
-      if (vs > vref) {
-        const float q = vref / vs;
-#pragma unroll
-        for (int b = 0; b < DB; ++b) o[b] *= q;
-        vref = vs;
-      }
       if (__ballot(mx > m + kDefer) != 0) {
         mx = fmaxf(mx, xor32(mx));
         const float mn = fmaxf(m, mx);
@@ -1244,8 +1254,7 @@ __global__ void __launch_bounds__(64 * RW * SLOTS, 2) kv8_prompt_kernel(const At
 #pragma unroll
         for (int b = 0; b < DB; ++b) o[b] *= al;
       }
-      float back;
-      const float vw = value_weight(poisoned ? 0.f : vs, vref, back), up = m == -INFINITY ? kBias : kBias - m;
+      const float up = m == -INFINITY ? kBias : kBias - m;
       if (poisoned) {                                    // NaN for the rows that see a key of it
 #pragma unroll
         for (int b = 0; b < 2; ++b)
