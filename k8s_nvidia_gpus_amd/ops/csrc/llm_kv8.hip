@@ -597,7 +597,8 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
 
 // ---------------------------------------------------------------- attention, both forms
 // The pages that queries at positions lo .. hi see, as a list: the first `sinks` ones, then those from
-// `first` on.
+// `first` on.  For one query each of them has a key that it sees (decode counts on it: the page's value scale
+// and poison are the row's).
 struct Seen {
   int nsink, first, n;
   __device__ __forceinline__ int page(int i) const { return i < nsink ? i : first + i - nsink; }
@@ -610,7 +611,7 @@ __host__ __device__ __forceinline__ Seen seen_pages(int lo, int hi, int span, in
   if (window > 0) {
     const int low = lo - window + 1;
     s.first = low > 0 ? low / kPage : 0;
-    if (s.first > last) s.first = last;
+    if (low >= end) s.first = last;                      // (no key of page low / kPage lies in the window)
     const int ns = sinks < end ? (sinks + kPage - 1) / kPage : last;
     s.nsink = ns < s.first ? ns : s.first;
   }

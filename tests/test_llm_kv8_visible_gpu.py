@@ -1,5 +1,5 @@
 """The 8-bit cache's attentions and pages that a row does not see: their scales and poison stay without
-effect on it, although other rows of the same call meet them.
+effect on it, although other rows of the same call, or other keys of the same span, meet them.
 
 Tolerance of an output element, A = sum_j p_j |v_j| over the row's n visible keys: half a step of the output's
 type; a weight's fp16 rounding, 2^-11 A, and scores, exponents and sums in fp32, 2^-12 A (chains of up to 64
@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from test_llm_kv8_gpu import CODES, DEV, KV, PAGE, dense, prompt_case, run_prompt   # noqa: F401
+from test_llm_kv8_gpu import CODES, DEV, KV, PAGE, dense, ints, prompt_case, run_prompt   # noqa: F401
 
 pytestmark = pytest.mark.gpu
 TOP = {"int8": 127.0, "e4m3": 448.0}
@@ -64,3 +64,22 @@ def test_prompt_a_large_page_behind_a_row(KV, code):   # noqa: F811
     cache, rows, q = prompt_case(KV, [0], [100], 8, 2, 128, code, torch.bfloat16, seed=81)
     cache.vs[rows[0][0]], cache.vs[rows[0][1]] = 2.0 ** -100, 2.0 ** 60
     check_rows(cache, rows[0], q, 0, 1 / math.sqrt(128), run_prompt(KV, cache, rows, q, [0], [100]), code)
+
+
+@pytest.mark.parametrize("poison", [float("nan"), 2.0 ** 60])
+@pytest.mark.parametrize("span,window,sinks", [(100, 190, 0), (100, 190, 5), (70, 300, 60), (70, 240, 0), (65, 299, 0)])
+def test_a_page_that_a_window_leaves_within_the_span(KV, poison, span, window, sinks):   # noqa: F811
+    """Position 300, keys below `span` only: the window begins in page 1, at or behind the span, or not."""
+    cache, rows, q = prompt_case(KV, [300], [1], 8, 2, 128, "int8", torch.bfloat16, seed=82)
+    seen = max(0, 300 - window + 1) < span
+    if not seen:
+        cache.vs[rows[0][1]] = poison
+    scale = 1 / math.sqrt(128)
+    for name in ("decode", "prompt"):
+        out = torch.full_like(q, 7.0)
+        if name == "decode":
+            KV.kv8_attn_decode(q, cache, ints(rows), ints([300]), out, scale, window=window, sinks=sinks, span=span)
+        else:
+            KV.kv8_attn_prompt(q, cache, ints(rows), ints([300]), ints([0, 1]), out, scale, window=window,
+                               sinks=sinks, span=span)
+        check_rows(cache, rows[0], q, 300, scale, out, "int8", window, sinks, span)
