@@ -640,10 +640,10 @@ __device__ __forceinline__ float score_factor(float ks, float c) {
 // were 0).
 // The weights p = 2^(s - m) go to the matrix instruction as fp16 p vs / vref, so that pages of unlike
 // scales add up in one accumulator; the sum of the plain p's takes the factor back (`back`).  A zero
-// page has zero codes: any weight will do.  A NaN scale stays.  What the rounding costs: 2^-12 of a
-// weight, and weights below 2^-32 (of the largest weight times the largest value scale) are lost.
-// The reference maximum lies up to 8 below the true one (rescaling is put off that long) and kBias above
-// the exponent's: weights reach from 2^15, under fp16's largest, down to 2^-31 of the largest's step.
+// page has zero codes: any weight will do.  A NaN scale stays.  What the rounding costs: 2^-11 of a weight,
+// and what is below 2^-32 of the largest weight times the largest value scale is lost.  For the reference
+// maximum lies up to 8 below the true one (rescaling is put off that long) and the exponents have kBias
+// added: the largest weight is 2^7 to 2^15, under fp16's largest, and half of fp16's least step is 2^-25.
 constexpr float kDefer = 8.f, kBias = 7.f;
 __device__ __forceinline__ float value_weight(float vs, float ratio, float& back) {   // ratio: vs / vref
   float lw = vs == 0.f ? 0.f : __builtin_amdgcn_logf(ratio);

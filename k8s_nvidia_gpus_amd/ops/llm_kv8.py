@@ -15,7 +15,8 @@ a sliding window has left behind can be freed.
 Both attentions take a sliding window and a number of first positions that stay visible (sinks): the
 query at position p sees key j when ``j <= p and (window == 0 or j > p - window or j < sinks)``.  A row
 that sees nothing is zero.  Softmax weights are rounded to fp16 after the value scales have been put on
-them, relative to the largest scale that the row sees: a value 2^-25 of the largest or less adds nothing.
+them: a weight times its page's value scale loses up to 2^-11 of itself, and where it is 2^-32 or less of the
+largest weight times the largest value scale that the row sees, it adds nothing to the output.
 
 Ragged sequences: ``cu`` (int32 [S + 1]) has the first row of each sequence, ``start`` (int32 [S]) its
 first position; rows at or behind ``cu[S]`` belong to none and their outputs stay as they were.  Lengths,
