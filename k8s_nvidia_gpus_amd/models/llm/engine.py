@@ -665,6 +665,9 @@ class Engine:
         """``tokens`` None: the tokens are the previous greedy step's ids of this batch size,
         still on the GPU (a chained step, ``decode_greedy_async``)."""
         T = len(positions)
+        fused = len(set(slots)) == len(slots)
+        # (raises before anything is enqueued: a copy from a pinned row must not be left without its event)
+        runs = self._runs_of(positions, slots) if self.kv8 is not None and not fused else None
         b = self._buffers(T)
         # one H2D copy per step from a pinned staging row (three synchronous pageable copies cost
         # ~3 x 10 us of idle GPU per token); the event guards the row against being rewritten
@@ -679,9 +682,8 @@ class Engine:
             b.host.copy_(torch.tensor([list(tokens), list(positions), list(slots)],
                                       dtype=torch.int32))
             b.meta.copy_(b.host, non_blocking=True)
-        fused = len(set(slots)) == len(slots)
-        if self.kv8 is not None and not fused:
-            b.runs_host.copy_(self._runs_of(positions, slots))
+        if runs is not None:
+            b.runs_host.copy_(runs)
             b.runs.copy_(b.runs_host, non_blocking=True)
         if b.host_evt is None:
             b.host_evt = torch.cuda.Event()

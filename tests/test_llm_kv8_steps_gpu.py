@@ -1,0 +1,22 @@
+"""Decode steps of the LLM engine on its 8-bit KV cache: refusals and buffers."""
+import pytest
+import torch
+
+from test_llm_kv8_engine_gpu import dev, engine, prompt, tiny_gguf   # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("call", ["decode", "decode_greedy", "decode_greedy_async"])
+def test_a_refused_step_leaves_the_steps_buffers_alone(dev, tiny_gguf, call):   # noqa: F811
+    eng = engine(tiny_gguf, dev, kv_type="int8")
+    eng.prefill(prompt(20, 1), 0)
+    eng.prefill(prompt(30, 2), 1)
+    eng.decode([3, 4], [20, 30], [0, 1])
+    torch.cuda.synchronize()
+    b = eng._bufs[2]
+    before = b.host.clone(), b.meta.clone(), b.runs.clone()
+    with pytest.raises(ValueError, match="consecutive"):
+        getattr(eng, call)([5, 6], [21, 21], [0, 0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip((b.host, b.meta, b.runs), before))
