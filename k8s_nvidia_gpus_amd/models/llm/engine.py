@@ -71,11 +71,12 @@ class StepBuffers:
     dxf: torch.Tensor       # its own input (x8/dx/sx) is still being read
     sxf: torch.Tensor
     qkv: torch.Tensor
-    qrot: torch.Tensor
-    po: torch.Tensor
-    pml: torch.Tensor
     t: torch.Tensor
     logits: torch.Tensor
+    # fp16 cache only: rotated queries and the attention's partials (chunks of max_ctx)
+    qrot: torch.Tensor = None
+    po: torch.Tensor = None
+    pml: torch.Tensor = None
     graphs: Dict[tuple, torch.cuda.CUDAGraph] = None   # keyed by (attention span, fused rope)
     ids: torch.Tensor = None         # int32 [T]: greedy next tokens (decode_greedy)
     meta: torch.Tensor = None        # int32 [3, T] on the GPU: tok / pos / slot are its rows
@@ -529,7 +530,6 @@ class Engine:
         if b is None:
             c, dev = self.cfg, self.device
             kmax = max(c.dim, c.ffn)
-            nsplit = self.max_ctx // self.LK.attn_chunk()
             f32 = dict(dtype=torch.float32, device=dev)
             meta = torch.zeros(3, T, dtype=torch.int32, device=dev)
             b = StepBuffers(
@@ -544,11 +544,14 @@ class Engine:
                 dx=torch.zeros(T, kmax // 32, **f32), sx=torch.zeros(T, kmax // 16, **f32),
                 x8f=torch.zeros(T, c.ffn, dtype=torch.int8, device=dev),
                 dxf=torch.zeros(T, c.ffn // 32, **f32), sxf=torch.zeros(T, c.ffn // 16, **f32),
-                qkv=torch.zeros(T, c.dim + 2 * c.kv_dim, **f32), qrot=torch.zeros(T, c.dim, **f32),
-                po=torch.zeros(T, c.heads, nsplit, c.head_dim, **f32),
-                pml=torch.zeros(T, c.heads, nsplit, 2, **f32), t=torch.zeros(T, c.ffn, **f32),
+                qkv=torch.zeros(T, c.dim + 2 * c.kv_dim, **f32), t=torch.zeros(T, c.ffn, **f32),
                 logits=torch.zeros(T, c.vocab, **f32))
-            if self.kv8 is not None:
+            if self.kv8 is None:
+                nsplit = self.max_ctx // self.LK.attn_chunk()
+                b.qrot = torch.zeros(T, c.dim, **f32)
+                b.po = torch.zeros(T, c.heads, nsplit, c.head_dim, **f32)
+                b.pml = torch.zeros(T, c.heads, nsplit, 2, **f32)
+            else:
                 cols = self.kv_pages.shape[1]
                 b.q16 = torch.zeros(T, c.heads, c.head_dim, dtype=torch.float16, device=dev)
                 b.pages = torch.zeros(T, cols, dtype=torch.int32, device=dev)
