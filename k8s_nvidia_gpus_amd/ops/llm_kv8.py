@@ -69,6 +69,9 @@ def _lib():
                 f.argtypes, f.restype = [ctypes.c_char_p, cf, vp, cl, vp], ci
                 f = getattr(lib, f"amdk8s_llm_kv8_{name}_work")
                 f.argtypes, f.restype = [ctypes.c_char_p], cl
+            if lib.amdk8s_llm_kv8_page() != PAGE:
+                raise RuntimeError(f"llm_kv8: the kernel library's pages have {lib.amdk8s_llm_kv8_page()} "
+                                   f"positions, not {PAGE}: built from other sources")
             _entries = lib
     return _entries
 
