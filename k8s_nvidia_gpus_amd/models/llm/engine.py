@@ -30,6 +30,7 @@ from __future__ import annotations
 
 import math
 import time
+import warnings
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -139,6 +140,9 @@ class Engine:
         # cache that is entered in its middle keeps its scale, and that scale (or poison) may come from the
         # positions that were cut off; a page begun anew forgets them.
         self.prefix_step = 1
+        if kv_type != "f16" and not self.gpu:
+            warnings.warn(f"kv_type {kv_type!r}: without a GPU the engine runs the reference maths, whose "
+                          "cache is not rounded")
         if kv_type != "f16" and self.gpu:
             from k8s_nvidia_gpus_amd.ops import llm_kv8 as KV
 

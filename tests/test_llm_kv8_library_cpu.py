@@ -1,4 +1,7 @@
-"""The 8-bit cache's entry points and the kernel library agree on the page size, or no call is made."""
+"""The 8-bit cache's entry points and the kernel library agree on the page size, or no call is made; an
+engine that cannot keep the cache in 8 bits says so."""
+import warnings
+
 import pytest
 
 from k8s_nvidia_gpus_amd.ops import llm_kv8 as KV
@@ -14,3 +17,16 @@ def test_another_page_size_is_refused(monkeypatch):
     with pytest.raises(RuntimeError, match="64 positions"):
         KV._lib()
     assert KV._entries is None
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_an_engine_without_a_gpu_says_that_its_cache_is_not_rounded(tmp_path, kind):
+    from k8s_nvidia_gpus_amd.models.llm import tiny
+    from k8s_nvidia_gpus_amd.models.llm.synthetic import load, write_synthetic_gguf
+
+    path = write_synthetic_gguf(str(tmp_path / "tiny.gguf"), tiny())
+    with pytest.warns(UserWarning, match="not rounded"):
+        load(path, device="cpu", max_ctx=256, kv_type=kind)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        load(path, device="cpu", max_ctx=256)
