@@ -46,7 +46,9 @@ the logits can differ in the last bits from an uncached prefill of the same prom
 admitted in the same iteration are prefilled together (one GEMM over all their rows), so the same
 holds with concurrent traffic: a seeded or greedy request can differ in the last bits, and rarely
 in a token, depending on which prompts arrived with it — ``--no-prompt-batch`` prefills every
-prompt alone for runs that must reproduce exactly.  Decode itself is batch-invariant.
+prompt alone for runs that must reproduce exactly.  Decode itself is batch-invariant with the fp16
+cache; with an 8-bit one (``--cache-type``) a step's attention is summed in parts that depend on the
+batch, so its last bits can differ with the sequences beside it.
 """
 from __future__ import annotations
 
@@ -1104,7 +1106,9 @@ def main(argv=None) -> int:
                     help="prompt tokens per chunk while nothing decodes (llama-server -b)")
     ap.add_argument("-ct", "--cache-type", choices=["f16", *KV8_TYPES], default="f16",
                     help="KV cache elements: int8 and e4m3 (8 bits and a scale for each 64 positions "
-                         "and head) halve its memory and the bytes a step at a long context reads")
+                         "and head) halve its memory and the bytes a step at a long context reads; "
+                         "e4m3 for models with a large key bias (int8 then rounds the other channels "
+                         "away); decode is not batch-invariant with either")
     ap.add_argument("-ngl", "--n-gpu-layers", type=int, default=999, help="accepted; all layers run on the GPU")
     ap.add_argument("-t", "--threads", type=int, default=0, help="accepted; the GPU does the work")
     ap.add_argument("--no-prompt-batch", action="store_true",

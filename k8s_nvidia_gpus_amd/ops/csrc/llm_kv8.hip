@@ -520,8 +520,8 @@ struct ReadArgs {
 };
 
 // One page of one sequence and KV head a block: keys row by row, values through byte transposes and LDS.
-// Memory-bound, four fifths of the bytes stores: 8 x 16384 positions 56 us, 5.1 TB/s; through the caches
-// (key codes in, rows out) 68.
+// Memory-bound, with 16-bit rows two thirds of the bytes stores: 8 x 16384 positions 56 us, 5.2 TB/s (a copy
+// reaches as much); through the caches (key codes in, rows out) 68.
 template <int D, bool FP8, int T>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
   typedef typename Elem<T>::type E;
@@ -710,10 +710,12 @@ __device__ __forceinline__ void put_q8(const AttnArgs& a, int t, long col, const
 // A page's keys are loaded as soon as the last page's have been used, and its values likewise: 16 KB in
 // flight a wave most of the time at half the registers of two buffers, so three waves fit a SIMD (two
 // buffers left one; 32 x 16000 with a window 140 us, this 61, with what follows 51).  ONCE: up to 16 heads
-// a KV head, so that no other workgroup reads the page; its values are loaded past the caches (8 x 32768
-// 44 -> 40 us, with the window 61 -> 57; with 128 heads on one KV head 14.5 -> 16.6).  Bound by the cache's
-// bytes: 8 x 32768 in e4m3 40 us, 5.2 TB/s, where a copy reaches 5.1; short contexts by launches (two, 2 to
-// 3 us each) and the chain position, page entry, page, join: 8 x 4096 13.4 us, 500 positions 8.1.
+// a KV head, so that no other workgroup of the row reads the page; its values are loaded past the caches
+// (8 x 32768 44 -> 40 us, with the window 61 -> 57; with 128 heads on one KV head 14.5 -> 16.6).  Pages that
+// sequences share are then fetched past them by each, which costs nothing: with three quarters of every row
+// shared 8 x 32000 35.1 us, through the caches 36.0; 32 x 4000 22.3 and 22.0.  Bound by the cache's bytes:
+// 8 x 32768 in e4m3 40 us, 5.3 TB/s, where a kernel that only reads reaches 6.5; short contexts by launches
+// (two, 2 to 3 us each) and the chain position, page entry, page, join: 8 x 4096 13.4 us, 500 positions 8.1.
 template <int D, bool FP8, int T, int NW, bool ONCE>
 __global__ void __launch_bounds__(64 * NW, 3) kv8_decode_kernel(const AttnArgs a) {
   constexpr int KH = D / 64, ND = D / 16;
@@ -1020,13 +1022,15 @@ __global__ void __launch_bounds__(64 * NW) kv8_join_kernel(const AttnArgs a) {
 // rescaling need one exchange (lane ^ 32).  The key of position p lies in LDS row p with bits 2 and 3
 // swapped, so that the score registers of a lane are, in order, the P operand's consecutive positions: P
 // never moves.
-// What bounds it: matrix and vector instructions of a SIMD's two waves hardly overlap (8192 rows at 0:
-// matrix cores busy 42 % of the time, vector units 48 %), and half of the vector time is the exponents;
-// three waves a SIMD took 12 % fewer cycles at a clock 11 % lower.
-// 8192 at 0 496 us, 970 TFLOP/s of visible pairs (a library product of two 8192 matrices reaches 1450);
-// 512 at 31488 250 us.  Tried and not taken: 64 rows a wave (twice the registers, one wave a SIMD: 660
-// us), the next page's scores ahead of this page's weights (580), pages turned to fp16 images in memory
-// once and loaded into LDS directly (503, and 284 for 512 at 31488), wave priorities (no change).
+// What bounds it: matrix and vector instructions of a SIMD's two waves hardly overlap as they are scheduled
+// here (8192 rows at 0: matrix cores busy 40 % of the time, vector units 46 %): both waves leave a page's
+// barrier at once and ask for the same unit in the same order.  Half of the vector time is the exponents;
+// three waves a SIMD took 12 % fewer cycles at a clock 11 % lower.  Waves half a page apart were not tried.
+// 8192 at 0 503 to 513 us, 950 TFLOP/s of visible pairs (a library product of two 8192 matrices reaches
+// 1450); 512 at 31488 252 to 256 us, its 224 workgroups on 256 CUs.  Tried and not taken, by the form that
+// took 496 us: 64 rows a wave (twice the registers, one wave a SIMD: 660 us), the next page's scores ahead of
+// this page's weights (580), pages turned to fp16 images in memory once and loaded into LDS directly (503,
+// and 284 for 512 at 31488), wave priorities (no change).
 __device__ __forceinline__ int swap23(int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); }
 
 // A tile's LDS image: key rows of 2 D bytes and value rows of 128 (64 positions of a dim) in fp16, each
@@ -1269,6 +1273,9 @@ __global__ void __launch_bounds__(64 * RW * SLOTS, 2) kv8_prompt_kernel(const At
 #pragma unroll
           for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(fmaf(sc[b][i], f, up));
       }
+      // The row's sum is one of the weights as they were rounded, in 32 bits: what rounding does to a weight
+      // then stands above and below the line.  With the unrounded weights, at the same speed, errors were up
+      // to 8 % larger (rms; 6 x 300: 1.14e-4 -> 1.22e-4 of outputs of 0.42) and a third at the worst.
       h8 pa[4];
       const h2 one = {(_Float16)1.f, (_Float16)1.f};
       float ls0 = 0.f, ls1 = 0.f;
@@ -1469,8 +1476,11 @@ struct DecodePlan {
 // 18.5); where it does not, one page is enough (1 x 4000 with one page a wave 9.1, with two 10.7).
 // Waves that would have two pages or more go 8 to a workgroup and half as many parts, if those fill three
 // quarters of the CUs: fewer partials (32 x 16000 with a window 57 -> 51, 64 x 4000 49 -> 45, 48 x 2000
-// 25 -> 20; with 160 of 256 CUs 60 -> 61; with one page a wave 9.2 -> 10.8).  Up to 8 pages run in one
-// workgroup of 8 waves, which needs no join: 500 positions 8.1 us against 9.2.
+// 25 -> 20; with 160 of 256 CUs 60 -> 61; with one page a wave 9.2 -> 10.8).  Those figures are of pages in
+// random order.  Where a row's pages follow one another and rows start at multiples of 2 MB, so that all parts
+// stream in step, 8 waves are the slower ones: 8 x 32000 54 to 62 us, 4 waves 50, in random order 50 and 49.
+// Up to 8 pages run in one workgroup of 8 waves, which needs no join: 500 positions 8.1 us against 9.2.
+// (A row's sums therefore depend, in their last bits, on how many rows and what span are beside it.)
 DecodePlan decode_plan(const AttnCall& c) {
   const long n = most_seen(c, 1);
   if (n <= 8) return {8, 1, 1};
@@ -1493,7 +1503,8 @@ struct PromptPlan {
   long units, parts;
 };
 // The workgroup's form and how many workgroups share a row block's pages, by what they take (microseconds,
-// measured at D 128): its start and end, partly hidden in rounds after the first; a page, 1.5 for 4 waves
+// measured at D 128, and taken for D 64 too: there the choice is the best form or within 4 % of it for 6 x 300
+// at 700, 128 to 2048 rows at 0, 512 at 512 and at 16000, and 9 % off at 4096 rows): its start and end, partly hidden in rounds after the first; a page, 1.5 for 4 waves
 // alone on their CU and 2.05 beside another workgroup (two fit), 1.95 for 8 waves of rows, 1.1 for 4 of
 // rows in two key slots (of either one fits); partial outputs cost a join launch and their bytes.  The
 // time is the longest row block's or that of the rounds over the chip, whichever is more; a causal chunk's

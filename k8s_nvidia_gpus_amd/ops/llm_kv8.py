@@ -12,6 +12,16 @@ a sliding window has left behind can be freed.
 * :func:`kv8_attn_decode` — attention of one token for each sequence;
 * :func:`kv8_attn_prompt` — causal attention of ragged prompt chunks.
 
+A decode step is fastest with a sequence's pages in no order: where they follow one another and sequences start
+at multiples of 2 MB, all parts of the launch stream in step (8 sequences at 32000 positions 54 to 62 us
+instead of 50).  How many sequences a step has, and its ``span``, decide how a row's pages are cut into sums:
+outputs depend on them in the last bits.
+
+An int8 key shares its step with its page and head: 1/127 to 2/127 of the largest channel.  Where a few key
+channels are far larger than the others (a key bias), the others lose: attention over random keys is off by
+2.1 % (rms) without such channels, 3.6 % with one of 10, 11 % of 30 and 26 % of 100 times the others' spread.
+e4m3 keeps 3.6 % whatever their size.
+
 Both attentions take a sliding window and a number of first positions that stay visible (sinks): the
 query at position p sees key j when ``j <= p and (window == 0 or j > p - window or j < sinks)``.  A row
 that sees nothing is zero.  Softmax weights are rounded to fp16 after the value scales have been put on
