@@ -804,7 +804,8 @@ class Engine:
         return GreedyStep(host=host, event=evt, buffers=b)
 
     def prefill(self, tokens: Sequence[int], slot: int, start: int = 0) -> torch.Tensor:
-        """Process prompt tokens of one sequence; returns the logits of its last token [vocab]."""
+        """Process prompt tokens of one sequence; returns the logits of its last token [vocab].
+        A sequence that was cut back is continued best at a multiple of ``prefix_step``."""
         P = len(tokens)
         if P == 0:
             raise ValueError("prefill: empty prompt")
